@@ -40,6 +40,9 @@ CE_MODE_NONE, CE_MODE_SUM, CE_MODE_MAX = 0, 1, 2
 CE_SCORE_DEFER = 4   # score_flags bit: leave the page scores to ce_decode_scores
 CE_DTYPE_NONE, CE_DTYPE_F32, CE_DTYPE_F64, CE_DTYPE_BF16 = 0, 1, 2, 3
 
+# bytes of one (unit, KV head) slice of a 4-bit pool: 16 tokens
+CE_KV4_SLICE_BYTES = 576
+
 # size of the static scratch behind ce_decode_attn_score_static
 CE_DECODE_STATIC_SCRATCH_BYTES = 32 << 20
 
@@ -86,6 +89,13 @@ SIGNATURES = {
     "ce_replay_workspace_bytes": (I64, [I32, I32]),
     "ce_replay_error": (C.c_int, [P, I64, I64, P, P, I64, P, I64, P, F32, I32, I32, I32, I32, I32, P, P,
                                   P, I64, P, P]),
+    "ce_kv4_write": (C.c_int, [P, I64, I64, P, I64, I64, P, I64, I32, I32, I32, P, P, I64, P, P]),
+    "ce_kv4_read": (C.c_int, [P, P, I64, P, I64, I32, I32, I32, P, I64, I64, I64, P, I64, I64, I64, P, P]),
+    "ce_kv4_decode_workspace_bytes": (I64, [I32, I64, I32, I32, I32]),
+    "ce_kv4_decode_attn_score": (C.c_int, [P, I64, I64, P, P, I64, P, P, P, I64, P, P, P, F32, I32, I32, I32,
+                                           I32, I32, P, I64, I32, P, I64, I64, P, I32, P, I64, P, P]),
+    "ce_window_decode": (C.c_int, [P, I64, I64, P, P, I64, P, P, P, I64, P, F32, I32, I32, I32, I32, I32, I32,
+                                   I32, P, I32, I64, I64, P, P, I64, P, P]),
     "ce_selftest_wait": (C.c_int, [I32, I64, P, P, P]),
     "ce_choose_workspace_bytes": (I64, [I32, I32, I32]),
     "ce_choose": (C.c_int, [P, P, I32, P, I32, P, I32, I32, I32, I32, I32, P, I32, P, P, P,
@@ -94,6 +104,10 @@ SIGNATURES = {
     "ce_boundary": (C.c_int, [P, I64, I32, P, I64, I32, P, P, P, I64, I32, P, I64, I64, I64,
                               P, P, I32, I32, I32, I32, I32, P, I32, P, P, P, I32, P, I32, P,
                               I32, I32, I32, I32, I32, P, P, I64, P, I64, I64, P, I64, P, P, P]),
+    "ce_kv4_boundary_workspace_bytes": (I64, [I32, I32, I32, I32, I32, I32, I32, I64]),
+    "ce_kv4_boundary": (C.c_int, [P, I64, I32, P, I64, I32, P, P, P, I64, I32, P, I64, I64, I64,
+                                  P, P, I32, I32, I32, I32, I32, P, I32, P, P, P, I32, P, I32, P,
+                                  I32, I32, I32, I32, I32, P, P, I64, P, I64, I64, P, I64, P, P, P]),
     "ce_gather_row_scores": (C.c_int, [P, I64, P, I64, P, P, P, I64, I64, I64, I32, I32, P,
                                        P, I32, I32, P, P, P]),
     "ce_reservoir_scores": (C.c_int, [P, I32, I32, I32, I32, U64, P, P]),

@@ -41,132 +41,50 @@
 #include <cstring>
 #include <mutex>
 
-#include "ce_common.cuh"
-#include "ce_host.h"
+#include "ce_decode.cuh"
 
 namespace ce {
 namespace decode {
 
-constexpr int D = 64;
-constexpr int GROUP = 8;
-constexpr int NCW = 8;                    // consumer warps
 constexpr int NPW = 4;                    // producer warps (stage k is issued by warp NCW + k % NPW)
 constexpr int THREADS = (NCW + NPW) * 32;
 constexpr int ROW_BYTES = D * 2;          // 128 B per (token, head) row
 constexpr int HALF_STAGE = NCW * 16 * ROW_BYTES;  // 16 KB of K (or V) per stage
 constexpr int STAGE_BYTES = 2 * HALF_STAGE;
 constexpr int NSTAGES = 6;
-constexpr int REC_ROWS = NCW * 8;         // virtual rows: warp w, head-row r
-constexpr int REC_FLOATS = REC_ROWS * D + 2 * REC_ROWS;
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 constexpr int SMEM_BYTES = NSTAGES * STAGE_BYTES + 1024 /*align*/ + 1024 /*barriers+misc*/;
 
-struct Params {
-  const __nv_bfloat16* q;
-  int64_t q_sb, q_sh;
-  const int32_t* kv_indptr;
-  const int32_t* kv_indices;
-  const int32_t* kv_tokens;
-  int64_t kv_capacity;
-  int64_t pool_units;
-  const float* sinks;
-  const int32_t* mode_of_row;
-  const int64_t* rows;
-  float scale_log2;
-  int bs, H, G;
-  float* scores;
-  int64_t score_sg;
-  int zero_new;
-  void* out;
-  int out_f32;
-  int64_t o_sb, o_sh;
-  float* lse_out;
-  int32_t* prefix;   // [bs + 1] stage prefix (written by CTA 0)
-  float* lse2;       // [bs, H] log2 normaliser per query head (for scores)
-  float* rec;        // [(bs + grid), REC_FLOATS]
-  float* ul;         // [kv_capacity, H] unit log-mass (log2 units) or null
-  float* tl;         // [kv_capacity * P, H] token logits (page_size > 1, MAX rows) or null
-  int32_t* err;
-};
+constexpr int MIN_STAGES_LOG2 = 2;        // at least 4 stages per CTA: the pipeline's depth
 
 __device__ __forceinline__ int stage_tokens(int G) { return 16 * (NCW / G); }
 
-// Partitions actually used: at least MIN_STAGES_PER_CTA stages each, so a
-// short batch is not spread thinner than the pipeline depth.
-constexpr int64_t MIN_STAGES_PER_CTA = 4;
-__device__ __forceinline__ int64_t eff_grid(int64_t S, int64_t launched) {
-  const int64_t want = (S + MIN_STAGES_PER_CTA - 1) / MIN_STAGES_PER_CTA;
-  return want < 1 ? 1 : (want < launched ? want : launched);
-}
-
-__device__ __forceinline__ int seq_tokens(const Params& p, int b, int P) {
-  if (p.kv_tokens) return max(0, p.kv_tokens[b]);
-  return max(0, (p.kv_indptr[b + 1] - p.kv_indptr[b]) * P);
-}
-
-__device__ __forceinline__ int seq_mode(const Params& p, int b) {
-  if (!p.mode_of_row) return CE_MODE_NONE;
-  const int64_t row = p.rows ? p.rows[b] : b;
-  return p.mode_of_row[row];
-}
-
-// Block-wide exclusive scan of one int64 per thread (THREADS threads).
-__device__ int64_t block_excl_scan(int64_t v, int64_t* sh, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) sh[warp] = x;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int64_t run = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
-      int64_t t = sh[w];
-      sh[w] = run;
-      run += t;
+// Stages of a sequence of n tokens.  WIN: only those that hold a visible
+// token, which are the first `head` stages (the first tokens) and, after
+// `skip` stages that are left out, the window's; the sequence's j-th stage
+// then starts at token (j + (j >= head ? skip : 0)) * ST.
+template <bool WIN>
+struct SeqStages {
+  int n = 0, nst = 0, head = 0, skip = 0, lo = 0, first = 0;
+  __device__ __forceinline__ SeqStages() {}
+  __device__ __forceinline__ SeqStages(const Params& p, int b, int P, int ST) {
+    n = seq_tokens(p, b, P);
+    nst = (n + ST - 1) / ST;
+    if constexpr (WIN) {
+      first = min(p.first, n);
+      lo = p.window < 0 ? 0 : max(0, n - p.window);   // first token of the window
+      head = (first + ST - 1) / ST;
+      skip = max(0, lo / ST - head);
+      nst -= skip;
     }
-    sh[31] = run;
   }
-  __syncthreads();
-  int64_t res = sh[warp] + x - v;
-  total = sh[31];
-  __syncthreads();
-  return res;
-}
+  __device__ __forceinline__ int at(int j) const { return WIN && j >= head ? j + skip : j; }
+  __device__ __forceinline__ bool visible(int t) const { return !WIN || t < first || t >= lo; }
+  // Whether any token of [t, t + k) is visible / every one is.
+  __device__ __forceinline__ bool some(int t, int k) const { return !WIN || t < first || t + k > lo; }
+  __device__ __forceinline__ bool every(int t, int k) const { return !WIN || t + k <= first || t >= lo; }
+};
 
-__device__ __forceinline__ int cta_of_stage(int64_t x, int64_t S, int64_t grid) {
-  return static_cast<int>(((x + 1) * grid - 1) / S);
-}
-
-// When there are fewer stages than CTAs some partitions are empty and leave
-// no record; a sequence's record range [k0, k1] may straddle them.
-__device__ __forceinline__ bool cta_has_work(int64_t k, int64_t S, int64_t grid) {
-  return (k * S) / grid < ((k + 1) * S) / grid;
-}
-
-__device__ __forceinline__ void store_out(const Params& p, int b, int h, int d, float v) {
-  const int64_t off = static_cast<int64_t>(b) * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d;
-  if (p.out_f32)
-    reinterpret_cast<float*>(p.out)[off] = v;
-  else
-    reinterpret_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
-}
-
-// A sequence with no tokens attends only to the sink: zero output.
-__device__ void empty_sequence(const Params& p, int b) {
-  for (int h = 0; h < p.H; ++h) {
-    for (int d = 0; d < D; ++d) store_out(p, b, h, d, 0.f);
-    const float s2 = p.sinks ? p.sinks[h] * LOG2E : -INFINITY;
-    p.lse2[static_cast<int64_t>(b) * p.H + h] = s2;
-    if (p.lse_out) p.lse_out[static_cast<int64_t>(b) * p.H + h] = s2 * LN2;
-  }
-}
-
-template <int P>
+template <int P, bool WIN>
 __global__ void __launch_bounds__(THREADS, 1)
     attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                 const Params p) {
@@ -200,16 +118,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int per = (bs + THREADS - 1) / THREADS;
   const int lo_b = min(bs, tid * per), hi_b = min(bs, lo_b + per);
   int64_t local = 0;
-  for (int b = lo_b; b < hi_b; ++b) local += (seq_tokens(p, b, P) + ST - 1) / ST;
+  for (int b = lo_b; b < hi_b; ++b) local += SeqStages<WIN>(p, b, P, ST).nst;
   int64_t S = 0;
   const int64_t excl = block_excl_scan(local, scan_sh, S);  // includes __syncthreads
-  const int64_t k = blockIdx.x, grid = eff_grid(S, gridDim.x);
+  const int64_t k = blockIdx.x, grid = eff_grid(S, gridDim.x, MIN_STAGES_LOG2);
   const int64_t S_lo = k < grid ? k * S / grid : S, S_hi = k < grid ? (k + 1) * S / grid : S;
   if (blockIdx.x == 0) {
     int64_t run = excl;
     for (int b = lo_b; b < hi_b; ++b) {
       p.prefix[b] = static_cast<int32_t>(run);
-      const int64_t n = (seq_tokens(p, b, P) + ST - 1) / ST;
+      const int64_t n = SeqStages<WIN>(p, b, P, ST).nst;
       run += n;
       if (n == 0) empty_sequence(p, b);   // no CTA will touch it
     }
@@ -225,7 +143,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (S_lo < S_hi && excl <= S_lo && S_lo < excl + local) {
     int64_t run = excl;
     for (int b = lo_b; b < hi_b; ++b) {
-      const int64_t n = (seq_tokens(p, b, P) + ST - 1) / ST;
+      const int64_t n = SeqStages<WIN>(p, b, P, ST).nst;
       if (S_lo < run + n) {
         start_sh[0] = b;
         start_sh[1] = static_cast<int>(run);
@@ -254,11 +172,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     // every 4 stages.)
     int issued = 0;
     int b = b_start, base = base_start;
-    int nst = 0, tok_b = 0;
+    SeqStages<WIN> sq;
     int64_t ip_b = 0;
     auto load_seq = [&](int bb) {
-      tok_b = seq_tokens(p, bb, P);
-      nst = (tok_b + ST - 1) / ST;
+      sq = SeqStages<WIN>(p, bb, P, ST);
       ip_b = p.kv_indptr[bb];
     };
     if (b < bs) load_seq(b);
@@ -269,14 +186,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     int64_t w0 = -1;
     int idx_cur = -2, idx_next = -2, idx_ahead = -2;
     for (int64_t x = S_lo; x < S_hi; ++x) {
-      while (x >= base + nst) {
-        base += nst;
+      while (x >= base + sq.nst) {
+        base += sq.nst;
         ++b;
         load_seq(b);
       }
       if (*abort_flag) break;
-      const int j = static_cast<int>(x - base);
-      const int ntok = min(ST, tok_b - j * ST);
+      const int j = sq.at(static_cast<int>(x - base));
+      const int ntok = min(ST, sq.n - j * ST);
       const int nunits = (ntok + P - 1) / P;
       const int64_t c0 = ip_b + static_cast<int64_t>(j) * UPS;
       if (w0 < 0 || c0 < w0 || c0 + nunits > w0 + 64) {
@@ -310,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int a = __shfl_sync(0xffffffffu, idx_cur, slot & 31);
       const int bn = __shfl_sync(0xffffffffu, idx_next, slot & 31);
       int unit = -1;
-      if (lane < nunits) {
+      if (lane < nunits && sq.some(j * ST + lane * P, P)) {
         const int v = (slot < 32) ? a : bn;
         if (v == -2) {
           flag_error(p.err, CE_EW_CAPACITY);
@@ -395,18 +312,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     int s = 0;
     uint32_t ph = 0;
     int b = b_start, base = base_start;
-    int nst = 0, tok_b = 0;
+    SeqStages<WIN> sq;
     int64_t ip_b = 0;
     auto load_seq = [&](int bb) {
-      tok_b = seq_tokens(p, bb, P);
-      nst = (tok_b + ST - 1) / ST;
+      sq = SeqStages<WIN>(p, bb, P, ST);
       ip_b = p.kv_indptr[bb];
     };
     if (b < bs) load_seq(b);
     bool aborted = false;
     for (int64_t x = S_lo; x < S_hi; ++x) {
-      while (x >= base + nst) {
-        base += nst;
+      while (x >= base + sq.nst) {
+        base += sq.nst;
         ++b;
         load_seq(b);
       }
@@ -433,8 +349,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           mode = CE_MODE_NONE;
         }
       }
-      const int j = static_cast<int>(x - base);
-      const int ntok = min(ST, tok_b - j * ST);
+      const int j = sq.at(static_cast<int>(x - base));
+      const int ntok = min(ST, sq.n - j * ST);
       const int cs = s;
       const uint32_t cph = ph;
       if (++s == NSTAGES) {
@@ -450,18 +366,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (aborted) continue;
       uint8_t* kst = smem + cs * STAGE_BYTES;
       uint8_t* vst = kst + HALF_STAGE;
-      if (ntok < tau0 + 16) {
-        // Zero V rows of tokens past the end so 0-probability * garbage stays 0.
+      if (ntok < tau0 + 16 || !sq.every(j * ST + tau0, 16)) {
+        // Zero V rows of tokens past the end (or outside the window) so
+        // 0-probability * garbage stays 0.
         for (int idx = lane; idx < 16 * 8; idx += 32) {
           const int tau = tau0 + (idx >> 3);
-          if (tau >= ntok)
+          if (tau >= ntok || !sq.visible(j * ST + tau))
             *reinterpret_cast<uint4*>(vst + row_of(tau) * ROW_BYTES + (idx & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      if (tau0 >= ntok) {
+      if (tau0 >= ntok || !sq.some(j * ST + tau0, 16)) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[cs]);
         continue;
@@ -481,7 +398,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
         mma_16816_full(sacc, kf[ks][0], kf[ks][1], kf[ks][2], kf[ks][3], qb[ks][0], qb[ks][1]);
-      const bool v_lo = tau0 + r < ntok, v_hi = tau0 + r + 8 < ntok;
+      const bool v_lo = tau0 + r < ntok && sq.visible(j * ST + tau0 + r);
+      const bool v_hi = tau0 + r + 8 < ntok && sq.visible(j * ST + tau0 + r + 8);
       float sv[4];
       sv[0] = v_lo ? sacc[0] * p.scale_log2 : -INFINITY;
       sv[1] = v_lo ? sacc[1] * p.scale_log2 : -INFINITY;
@@ -855,7 +773,7 @@ __global__ void __launch_bounds__(CB_THREADS, SB == 1 ? 4 : 2) combine_kernel(co
   const Params& p = cp.a;
   const int bs = p.bs, H = p.H, G = p.G, C = cp.chunks;
   const int64_t S = p.prefix[bs];
-  const int64_t grid = eff_grid(S, cp.grid);
+  const int64_t grid = eff_grid(S, cp.grid, p.min_log2);
   const int hgroups = H / GROUP;
   const int64_t ntasks = static_cast<int64_t>(bs) * hgroups * C;
   __shared__ float sh_m[GROUP * CB_THREADS], sh_l[GROUP * CB_THREADS];
@@ -976,28 +894,46 @@ int combine_chunks(int bs, int H, int sms) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(c, CB_MAX_CHUNKS)));
 }
 
-struct DecodeLayout {
-  size_t prefix, lse2, rec, ul, tl, total;
-};
+}  // namespace
 
-DecodeLayout decode_layout(int bs, int64_t cap, int H, int P, int flags, int grid) {
+host::DecodeLayout ce::host::decode_layout(int bs, int64_t cap, int H, int P, int flags, int grid) {
   DecodeLayout L{};
   size_t off = 0;
   L.prefix = off;
   off += align256(sizeof(int32_t) * (bs + 1));
   L.lse2 = off;
   off += align256(sizeof(float) * (size_t)bs * H);
-  L.rec = off;
-  off += align256(sizeof(float) * (size_t)(bs + grid) * REC_FLOATS);
   L.ul = off;
   if (flags & 3) off += align256(sizeof(float) * (size_t)cap * H);
   L.tl = off;
   if ((flags & 2) && P > 1) off += align256(sizeof(float) * (size_t)cap * P * H);
+  L.rec = off;
+  off += align256(sizeof(float) * (size_t)(bs + grid) * REC_FLOATS);
   L.total = off;
   return L;
 }
 
-}  // namespace
+int ce::host::launch_combine(const Params& p, int grid, int P, bool defer, cudaStream_t st) {
+  const int sms = sm_count();
+  CombineParams cp{p, grid, P, defer ? 1 : 0, combine_chunks(p.bs, p.H, sms)};
+  const int64_t tasks = static_cast<int64_t>(p.bs) * (p.H / GROUP) * cp.chunks;
+  const int cb_grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tasks, 4LL * sms)));
+  // Fewer (sequence, KV head) pairs than SMs: each head has many record slots
+  // (up to one per CTA and warp group) and the tasks are chunks of few
+  // sequences -- the wide variant's batched loads win.
+  // A deferred decode's page scores run beside the next layer's attention
+  // kernel (195 KB of shared memory per CTA): keep SMs at the largest carveout.
+  const bool wide = static_cast<int64_t>(p.bs) * (p.H / GROUP) < sms;
+  if (wide) {
+    if (defer && !set_max_shared_carveout(combine_kernel<CB_SLOT_BATCH_WIDE>)) return fail(CE_ERR_CUDA, "carveout attr");
+    combine_kernel<CB_SLOT_BATCH_WIDE><<<cb_grid, CB_THREADS, 0, st>>>(cp);
+  } else {
+    if (defer && !set_max_shared_carveout(combine_kernel<1>)) return fail(CE_ERR_CUDA, "carveout attr");
+    combine_kernel<1><<<cb_grid, CB_THREADS, 0, st>>>(cp);
+  }
+  if (cudaPeekAtLastError() != cudaSuccess) return fail_cuda("combine_kernel launch");
+  return CE_OK;
+}
 
 extern "C" int64_t ce_decode_workspace_bytes(int32_t bs, int64_t kv_capacity, int32_t num_q_heads,
                                              int32_t num_kv_heads, int32_t page_size,
@@ -1006,21 +942,29 @@ extern "C" int64_t ce_decode_workspace_bytes(int32_t bs, int64_t kv_capacity, in
   if (bs < 0 || kv_capacity < 0 || num_q_heads <= 0 || page_size <= 0) return -1;
   const int grid = host::sm_count();
   if (grid <= 0) return -1;
-  return (int64_t)decode_layout(bs, kv_capacity, num_q_heads, page_size, score_flags, grid).total;
+  return (int64_t)host::decode_layout(bs, kv_capacity, num_q_heads, page_size, score_flags, grid).total;
 }
 
-extern "C" int ce_decode_attn_score(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool,
-                                    const void* v_pool, int64_t pool_units,
-                                    const int32_t* kv_indptr, const int32_t* kv_indices,
-                                    const int32_t* kv_tokens, int64_t kv_capacity,
-                                    const float* sinks, const int32_t* mode_of_row,
-                                    const int64_t* rows, float sm_scale, int32_t bs,
-                                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                                    int32_t page_size, float* scores, int64_t score_sg,
-                                    int32_t zero_new, void* out, int32_t out_f32, int64_t o_sb,
-                                    int64_t o_sh, float* lse_out, int32_t score_flags,
-                                    void* workspace, int64_t workspace_bytes, int32_t* err,
-                                    void* stream) {
+namespace {
+
+// WIN: only the window's tokens and the first ones are visible, and nothing is scored.
+template <int P, bool WIN>
+int launch_attn(int grid, const CUtensorMap& kmap, const CUtensorMap& vmap, const Params& p, cudaStream_t st) {
+  if (!host::set_smem(attn_kernel<P, WIN>, SMEM_BYTES)) return host::fail(CE_ERR_CUDA, "smem attr");
+  attn_kernel<P, WIN><<<grid, THREADS, SMEM_BYTES, st>>>(kmap, vmap, p);
+  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("attn_kernel launch");
+  return CE_OK;
+}
+
+template <bool WIN>
+int decode_call(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool, const void* v_pool,
+                int64_t pool_units, const int32_t* kv_indptr, const int32_t* kv_indices,
+                const int32_t* kv_tokens, int64_t kv_capacity, const float* sinks, const int32_t* mode_of_row,
+                const int64_t* rows, float sm_scale, int32_t bs, int32_t num_q_heads, int32_t num_kv_heads,
+                int32_t head_dim, int32_t page_size, int32_t window, int32_t first, float* scores,
+                int64_t score_sg, int32_t zero_new, void* out, int32_t out_f32, int64_t o_sb, int64_t o_sh,
+                float* lse_out, int32_t score_flags, void* workspace, int64_t workspace_bytes, int32_t* err,
+                void* stream) {
   if (bs < 0 || pool_units < 0 || kv_capacity < 0) return host::fail(CE_ERR_ARG, "negative size");
   if (head_dim != D) return host::fail(CE_ERR_UNSUPPORTED, "head_dim must be 64");
   if (num_kv_heads <= 0 || num_q_heads != GROUP * num_kv_heads || NCW % num_kv_heads != 0)
@@ -1038,7 +982,7 @@ extern "C" int ce_decode_attn_score(const void* q, int64_t q_sb, int64_t q_sh, c
   if ((q_sh | q_sb) & 1) return host::fail(CE_ERR_ARG, "q strides must be even");
   const int grid = host::sm_count();
   if (grid <= 0) return host::fail(CE_ERR_CUDA, "no device");
-  DecodeLayout L = decode_layout(bs, kv_capacity, num_q_heads, page_size, score_flags, grid);
+  host::DecodeLayout L = host::decode_layout(bs, kv_capacity, num_q_heads, page_size, score_flags, grid);
   if (workspace_bytes < (int64_t)L.total) return host::fail(CE_ERR_WORKSPACE, "decode workspace too small");
 
   CUtensorMap kmap, vmap;
@@ -1079,44 +1023,61 @@ extern "C" int ce_decode_attn_score(const void* q, int64_t q_sb, int64_t q_sh, c
   p.rec = reinterpret_cast<float*>(ws + L.rec);
   p.ul = (score_flags & 3) ? reinterpret_cast<float*>(ws + L.ul) : nullptr;
   p.tl = ((score_flags & 2) && page_size > 1) ? reinterpret_cast<float*>(ws + L.tl) : nullptr;
+  p.min_log2 = MIN_STAGES_LOG2;
+  p.window = window;
+  p.first = first;
   p.err = err;
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (page_size == 16) {
-    if (!host::set_smem(attn_kernel<16>, SMEM_BYTES)) return host::fail(CE_ERR_CUDA, "smem attr");
-    attn_kernel<16><<<grid, THREADS, SMEM_BYTES, st>>>(kmap, vmap, p);
-  } else {
-    if (!host::set_smem(attn_kernel<1>, SMEM_BYTES)) return host::fail(CE_ERR_CUDA, "smem attr");
-    attn_kernel<1><<<grid, THREADS, SMEM_BYTES, st>>>(kmap, vmap, p);
-  }
-  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("attn_kernel launch");
-  const bool defer = (score_flags & CE_SCORE_DEFER) != 0;
-  CombineParams cp{p, grid, page_size, defer ? 1 : 0, combine_chunks(bs, num_q_heads, grid)};
-  // A deferred decode's page scores run beside the next layer's attention
-  // kernel (195 KB of shared memory per CTA): keep SMs at the largest carveout.
-  const int64_t tasks = static_cast<int64_t>(bs) * (num_q_heads / GROUP) * cp.chunks;
-  const int cb_grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tasks, 4LL * grid)));
-  // Fewer (sequence, KV head) pairs than attention CTAs: each head has many
-  // record slots (up to one per CTA and warp group) and the tasks are chunks
-  // of few sequences -- the wide variant's batched loads win.
-  const bool wide = static_cast<int64_t>(bs) * (num_q_heads / GROUP) < grid;
-  if (wide) {
-    if (defer && !host::set_max_shared_carveout(combine_kernel<CB_SLOT_BATCH_WIDE>))
-      return host::fail(CE_ERR_CUDA, "carveout attr");
-    combine_kernel<CB_SLOT_BATCH_WIDE><<<cb_grid, CB_THREADS, 0, st>>>(cp);
-  } else {
-    if (defer && !host::set_max_shared_carveout(combine_kernel<1>)) return host::fail(CE_ERR_CUDA, "carveout attr");
-    combine_kernel<1><<<cb_grid, CB_THREADS, 0, st>>>(cp);
-  }
-  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("combine_kernel launch");
-  return CE_OK;
+  const int launched = page_size == 16 ? launch_attn<16, WIN>(grid, kmap, vmap, p, st)
+                                       : launch_attn<1, WIN>(grid, kmap, vmap, p, st);
+  if (launched != CE_OK) return launched;
+  return host::launch_combine(p, grid, page_size, (score_flags & CE_SCORE_DEFER) != 0, st);
+}
+
+}  // namespace
+
+extern "C" int ce_decode_attn_score(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool,
+                                    const void* v_pool, int64_t pool_units,
+                                    const int32_t* kv_indptr, const int32_t* kv_indices,
+                                    const int32_t* kv_tokens, int64_t kv_capacity,
+                                    const float* sinks, const int32_t* mode_of_row,
+                                    const int64_t* rows, float sm_scale, int32_t bs,
+                                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t page_size, float* scores, int64_t score_sg,
+                                    int32_t zero_new, void* out, int32_t out_f32, int64_t o_sb,
+                                    int64_t o_sh, float* lse_out, int32_t score_flags,
+                                    void* workspace, int64_t workspace_bytes, int32_t* err,
+                                    void* stream) {
+  return decode_call<false>(q, q_sb, q_sh, k_pool, v_pool, pool_units, kv_indptr, kv_indices, kv_tokens, kv_capacity,
+                            sinks, mode_of_row, rows, sm_scale, bs, num_q_heads, num_kv_heads, head_dim, page_size,
+                            -1, 0, scores, score_sg, zero_new, out, out_f32, o_sb, o_sh, lse_out, score_flags,
+                            workspace, workspace_bytes, err, stream);
+}
+
+extern "C" int ce_window_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool, const void* v_pool,
+                                int64_t pool_units, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                const int32_t* kv_tokens, int64_t kv_capacity, const float* sinks, float sm_scale,
+                                int32_t bs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t page_size, int32_t window, int32_t first, void* out, int32_t out_f32,
+                                int64_t o_sb, int64_t o_sh, float* lse_out, void* workspace,
+                                int64_t workspace_bytes, int32_t* err, void* stream) {
+  if (window == 0 || window < -1 || first < 0)
+    return host::fail(CE_ERR_ARG, "ce_window_decode: window must be at least 1 (or -1: none), first at least 0");
+  if (bs > 0 && (!kv_tokens || (reinterpret_cast<uintptr_t>(q) & 3)))
+    return host::fail(CE_ERR_ARG, "ce_window_decode: kv_tokens missing or q not 4-byte aligned");
+  return decode_call<true>(q, q_sb, q_sh, k_pool, v_pool, pool_units, kv_indptr, kv_indices, kv_tokens, kv_capacity,
+                           sinks, nullptr, nullptr, sm_scale, bs, num_q_heads, num_kv_heads, head_dim, page_size,
+                           window, first, nullptr, 0, 0, out, out_f32, o_sb, o_sh, lse_out, 0, workspace,
+                           workspace_bytes, err, stream);
 }
 
 int ce::host::decode_prepare_device() {
   // cudaFuncGetAttributes loads a kernel under lazy module loading; the
   // shared-memory attribute is the one the first launch would set.
   cudaFuncAttributes a;
-  if (!host::set_smem(attn_kernel<16>, SMEM_BYTES) || !host::set_smem(attn_kernel<1>, SMEM_BYTES) ||
+  if (!host::set_smem(attn_kernel<16, false>, SMEM_BYTES) || !host::set_smem(attn_kernel<1, false>, SMEM_BYTES) ||
+      !host::set_smem(attn_kernel<16, true>, SMEM_BYTES) || !host::set_smem(attn_kernel<1, true>, SMEM_BYTES) ||
       cudaFuncGetAttributes(&a, combine_kernel<1>) != cudaSuccess ||
       cudaFuncGetAttributes(&a, combine_kernel<CB_SLOT_BATCH_WIDE>) != cudaSuccess)
     return host::fail_cuda("decode kernels: set-up");
@@ -1140,7 +1101,7 @@ extern "C" int ce_decode_scores(const int32_t* kv_indptr, const int32_t* kv_indi
   if (page_size > 1 && !kv_tokens) return host::fail(CE_ERR_ARG, "kv_tokens required for page_size > 1");
   const int grid = host::sm_count();
   if (grid <= 0) return host::fail(CE_ERR_CUDA, "no device");
-  DecodeLayout L = decode_layout(bs, kv_capacity, num_q_heads, page_size, score_flags, grid);
+  host::DecodeLayout L = host::decode_layout(bs, kv_capacity, num_q_heads, page_size, score_flags, grid);
   if (workspace_bytes < (int64_t)L.total) return host::fail(CE_ERR_WORKSPACE, "decode workspace too small");
   Params p{};
   p.kv_indptr = kv_indptr;

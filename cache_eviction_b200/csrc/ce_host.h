@@ -57,5 +57,9 @@ int select_prepare_device();
 int fill_prepare_device();
 int pool_prepare_device();
 
+// The same for the 4-bit kernels (ce_kv4.cu, ce_kv4_decode.cu).
+int kv4_prepare_device();
+int kv4_copy_prepare_device();
+
 }  // namespace host
 }  // namespace ce

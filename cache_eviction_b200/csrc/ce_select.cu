@@ -25,6 +25,7 @@
 
 #include "ce_common.cuh"
 #include "ce_host.h"
+#include "ce_kv4.cuh"
 
 namespace ce {
 namespace sel {
@@ -1167,6 +1168,7 @@ struct BParams {
   const float* gscores;
   int GH;
   int live, max_cols, max_width, nw;
+  int slice; // bytes of one unit's K or V of one head
   int ch;   // middle survivors per compaction chunk (chunk_items)
   // workspace
   uint64_t* kv;
@@ -2004,7 +2006,7 @@ __global__ void __launch_bounds__(T) brecord_kernel(const BParams p) {
 // copied together (copy_items).
 constexpr int CH_PAGED = 8;
 constexpr int CH_SMALL = 32;
-__host__ __device__ __forceinline__ int chunk_items(int P) { return P * 128 >= 2048 ? CH_PAGED : CH_SMALL; }
+__host__ __device__ __forceinline__ int chunk_items(int slice) { return slice >= 2048 ? CH_PAGED : CH_SMALL; }
 
 struct Chunk {
   int i, l, g, j;         // this lane's item
@@ -2043,10 +2045,10 @@ __device__ __forceinline__ bool chunk_hazard(const BParams& p, const Chunk& c) {
   return cr >= 0 && cr < c.W && cr != c.j;
 }
 
+// The slice (`bytes` of K or V of one unit and KV head) of a layer's pool.
 __device__ __forceinline__ uint8_t* unit_ptr(const uint64_t* layers, int l, int unit, int g, int G,
-                                             int P) {
-  return reinterpret_cast<uint8_t*>(layers[l]) +
-         (static_cast<int64_t>(unit) * G + g) * static_cast<int64_t>(P) * 128;
+                                             int bytes) {
+  return reinterpret_cast<uint8_t*>(layers[l]) + (static_cast<int64_t>(unit) * G + g) * bytes;
 }
 
 // Copy one head slice of K and of V (bytes each) with the warp: every lane
@@ -2134,7 +2136,7 @@ __global__ void __launch_bounds__(256, SMALL ? 4 : 2) bgather_kernel(const BPara
   const int lane = threadIdx.x & 31;
   const uint32_t nchunks = launch_chunks(p, nr, nl);
   const uint32_t nwarps = gridDim.x * (blockDim.x >> 5);
-  const int bytes = p.P * 128;
+  const int bytes = p.slice;
   for (uint32_t wi = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); wi < nchunks; wi += nwarps) {
     const Chunk c = decode_chunk(p, wi, r0, l0, nl, lane);
     int src = -1;
@@ -2155,8 +2157,8 @@ __global__ void __launch_bounds__(256, SMALL ? 4 : 2) bgather_kernel(const BPara
       copy_items(hmask, bytes, lane,
                  [&](int k, const uint8_t*& sk, const uint8_t*& sv, uint8_t*& dk, uint8_t*& dv) {
                    const int s = max(__shfl_sync(0xffffffffu, src, k), 0);
-                   sk = unit_ptr(p.k_layers, c.l, s, c.g, p.G, p.P);
-                   sv = unit_ptr(p.v_layers, c.l, s, c.g, p.G, p.P);
+                   sk = unit_ptr(p.k_layers, c.l, s, c.g, p.G, bytes);
+                   sv = unit_ptr(p.v_layers, c.l, s, c.g, p.G, bytes);
                    dk = p.hazard + (item0 + k) * 2 * bytes;
                    dv = dk + bytes;
                  });
@@ -2167,8 +2169,8 @@ __global__ void __launch_bounds__(256, SMALL ? 4 : 2) bgather_kernel(const BPara
       const int s = __shfl_sync(0xffffffffu, src, k);
       const int64_t it = __shfl_sync(0xffffffffu, c.item, k);
       uint8_t* scr = p.hazard + it * 2 * bytes;
-      copy_pair(scr, scr + bytes, unit_ptr(p.k_layers, c.l, s, c.g, p.G, p.P),
-                unit_ptr(p.v_layers, c.l, s, c.g, p.G, p.P), bytes, lane);
+      copy_pair(scr, scr + bytes, unit_ptr(p.k_layers, c.l, s, c.g, p.G, bytes),
+                unit_ptr(p.v_layers, c.l, s, c.g, p.G, bytes), bytes, lane);
     }
   }
 }
@@ -2181,7 +2183,7 @@ __global__ void __launch_bounds__(256, SMALL ? 4 : 2) bscatter_kernel(const BPar
   const int lane = threadIdx.x & 31;
   const uint32_t nchunks = launch_chunks(p, nr, nl);
   const uint32_t nwarps = gridDim.x * (blockDim.x >> 5);
-  const int bytes = p.P * 128;
+  const int bytes = p.slice;
   for (uint32_t wi = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); wi < nchunks; wi += nwarps) {
     const Chunk c = decode_chunk(p, wi, r0, l0, nl, lane);
     int src = -1, dst = -1;
@@ -2208,10 +2210,10 @@ __global__ void __launch_bounds__(256, SMALL ? 4 : 2) bscatter_kernel(const BPar
                    const int d = max(__shfl_sync(0xffffffffu, dst, k), 0);
                    const bool h = __shfl_sync(0xffffffffu, hz, k);
                    const uint8_t* scr = p.hazard + (item0 + k) * 2 * bytes;
-                   sk = h ? scr : unit_ptr(p.k_layers, c.l, s, c.g, p.G, p.P);
-                   sv = h ? scr + bytes : unit_ptr(p.v_layers, c.l, s, c.g, p.G, p.P);
-                   dk = unit_ptr(p.k_layers, c.l, d, c.g, p.G, p.P);
-                   dv = unit_ptr(p.v_layers, c.l, d, c.g, p.G, p.P);
+                   sk = h ? scr : unit_ptr(p.k_layers, c.l, s, c.g, p.G, bytes);
+                   sv = h ? scr + bytes : unit_ptr(p.v_layers, c.l, s, c.g, p.G, bytes);
+                   dk = unit_ptr(p.k_layers, c.l, d, c.g, p.G, bytes);
+                   dv = unit_ptr(p.v_layers, c.l, d, c.g, p.G, bytes);
                  });
       continue;
     }
@@ -2221,9 +2223,9 @@ __global__ void __launch_bounds__(256, SMALL ? 4 : 2) bscatter_kernel(const BPar
       const int d = __shfl_sync(0xffffffffu, dst, k);
       const bool h = __shfl_sync(0xffffffffu, hz, k);
       const int64_t it = __shfl_sync(0xffffffffu, c.item, k);
-      const uint8_t* ks = h ? p.hazard + it * 2 * bytes : unit_ptr(p.k_layers, c.l, s, c.g, p.G, p.P);
-      const uint8_t* vs = h ? p.hazard + it * 2 * bytes + bytes : unit_ptr(p.v_layers, c.l, s, c.g, p.G, p.P);
-      copy_pair(unit_ptr(p.k_layers, c.l, d, c.g, p.G, p.P), unit_ptr(p.v_layers, c.l, d, c.g, p.G, p.P), ks, vs,
+      const uint8_t* ks = h ? p.hazard + it * 2 * bytes : unit_ptr(p.k_layers, c.l, s, c.g, p.G, bytes);
+      const uint8_t* vs = h ? p.hazard + it * 2 * bytes + bytes : unit_ptr(p.v_layers, c.l, s, c.g, p.G, bytes);
+      copy_pair(unit_ptr(p.k_layers, c.l, d, c.g, p.G, bytes), unit_ptr(p.v_layers, c.l, d, c.g, p.G, bytes), ks, vs,
                 bytes, lane);
     }
   }
@@ -2402,9 +2404,13 @@ BLayout boundary_layout(int R, int L, int G, int max_cols, int64_t hazard_bytes)
   return b;
 }
 
-int64_t hazard_per_layer(int R, int G, int max_width, int P) {
-  return static_cast<int64_t>(R) * G * max_width * 2 * P * 128;
+int64_t hazard_per_layer(int R, int G, int max_width, int slice) {
+  return static_cast<int64_t>(R) * G * max_width * 2 * slice;
 }
+
+// Bytes of a (unit, head) slice of a pool: 16-bit rows of 64, or the 4-bit
+// pages of ce_kv4.cuh.  Compaction moves slices whole, whatever they hold.
+int slice_bytes(bool four_bit, int page_size) { return four_bit ? kv4::SLICE : page_size * 128; }
 
 int sel_smem(int nw) { return nw * 8; }
 constexpr int kLargeSmemMax = 220 * 1024;   // dynamic shared memory a large-segment launch may use
@@ -2474,18 +2480,31 @@ extern "C" int ce_choose(const int32_t* pos, const int32_t* ncols, int32_t n_col
   return CE_OK;
 }
 
+namespace {
+int64_t boundary_bytes(bool four_bit, int32_t num_rows, int32_t layers, int32_t kv_heads, int32_t head_dim,
+                       int32_t page_size, int32_t max_cols, int32_t max_width, int64_t hazard_bytes) {
+  if (num_rows < 0 || layers <= 0 || kv_heads <= 0 || head_dim != 64 || page_size <= 0 || max_cols < 0 ||
+      (four_bit && page_size != kv4::P))
+    return -1;
+  const int width = (max_width > 0 && max_width < max_cols) ? max_width : max_cols;
+  const int64_t one = hazard_per_layer(1, kv_heads, width, slice_bytes(four_bit, page_size));   // one row of one layer
+  const int64_t hz = hazard_bytes < one ? one : hazard_bytes;
+  return static_cast<int64_t>(boundary_layout(num_rows, layers, kv_heads, max_cols, hz).total);
+}
+}  // namespace
+
 extern "C" int64_t ce_boundary_workspace_bytes(int32_t num_rows, int32_t layers, int32_t kv_heads,
                                                int32_t head_dim, int32_t page_size,
                                                int32_t max_cols, int32_t max_width,
                                                int32_t global_heads, int64_t hazard_bytes) {
   (void)global_heads;
-  if (num_rows < 0 || layers <= 0 || kv_heads <= 0 || head_dim != 64 || page_size <= 0 ||
-      max_cols < 0)
-    return -1;
-  const int width = (max_width > 0 && max_width < max_cols) ? max_width : max_cols;
-  const int64_t one = hazard_per_layer(1, kv_heads, width, page_size);   // one row of one layer
-  const int64_t hz = hazard_bytes < one ? one : hazard_bytes;
-  return static_cast<int64_t>(boundary_layout(num_rows, layers, kv_heads, max_cols, hz).total);
+  return boundary_bytes(false, num_rows, layers, kv_heads, head_dim, page_size, max_cols, max_width, hazard_bytes);
+}
+
+extern "C" int64_t ce_kv4_boundary_workspace_bytes(int32_t num_rows, int32_t layers, int32_t kv_heads,
+                                                   int32_t head_dim, int32_t page_size, int32_t max_cols,
+                                                   int32_t max_width, int64_t hazard_bytes) {
+  return boundary_bytes(true, num_rows, layers, kv_heads, head_dim, page_size, max_cols, max_width, hazard_bytes);
 }
 
 static int boundary_params(BParams& p, int32_t* table, int64_t table_stride, int32_t table_width,
@@ -2545,7 +2564,8 @@ extern "C" int ce_gather_row_scores(const int32_t* table, int64_t table_stride,
   return CE_OK;
 }
 
-extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_width,
+namespace {
+int boundary_call(bool four_bit, int32_t* table, int64_t table_stride, int32_t table_width,
                            int32_t* req_to_unit, int64_t r2u_stride, int32_t r2u_width,
                            int32_t* frontier, int32_t* count, int32_t* pos,
                            int64_t pos_row_stride, int32_t pos_cap, float* scores,
@@ -2567,6 +2587,7 @@ extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_w
   if (record_delta && (!record_counts || record_stride < max_cols))
     return host::fail(CE_ERR_ARG, "retention record needs counts and a row stride >= max_cols");
   if (head_dim != 64) return host::fail(CE_ERR_UNSUPPORTED, "head_dim must be 64");
+  if (four_bit && page_size != kv4::P) return host::fail(CE_ERR_UNSUPPORTED, "4-bit pages hold 16 tokens");
   if (num_rows == 0) return CE_OK;
   if (!table || !req_to_unit || !frontier || !count || !pos || !scores || !k_layers || !v_layers ||
       !rows || !params || !result || !workspace)
@@ -2578,7 +2599,8 @@ extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_w
   const int nw = (max_n + 31) / 32;
   if (sel_smem(nw) > 200 * 1024) return host::fail(CE_ERR_UNSUPPORTED, "max_n too large");
   const int width = (max_width > 0 && max_width < max_cols) ? max_width : max_cols;
-  const int64_t one = hazard_per_layer(1, kv_heads, width, page_size);   // one row of one layer
+  const int slice = slice_bytes(four_bit, page_size);
+  const int64_t one = hazard_per_layer(1, kv_heads, width, slice);   // one row of one layer
   const int64_t hz = hazard_bytes < one ? one : hazard_bytes;
   const BLayout Lo = boundary_layout(num_rows, layers, kv_heads, max_cols, hz);
   if (workspace_bytes < static_cast<int64_t>(Lo.total))
@@ -2589,7 +2611,8 @@ extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_w
                   score_head_stride, pool_units, layers, kv_heads, page_size, rows, params,
                   num_rows, max_cols, max_n);
   p.max_width = width;
-  p.ch = chunk_items(page_size);
+  p.slice = slice;
+  p.ch = chunk_items(slice);
   p.k_layers = k_layers;
   p.v_layers = v_layers;
   p.head_offset = head_offset;
@@ -2667,12 +2690,12 @@ extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_w
   // of as many layers as fit, or fewer rows of one layer).  Splitting further
   // to keep the staged copies in L2 was measured slower: the extra launches
   // cost more than the DRAM round trip they save.
-  const int64_t row_layer = hazard_per_layer(1, kv_heads, width, page_size);
+  const int64_t row_layer = hazard_per_layer(1, kv_heads, width, slice);
   const int rows_per = static_cast<int>(std::min<int64_t>(num_rows, std::max<int64_t>(1, hz / row_layer)));
   const int group = static_cast<int>(
       std::min<int64_t>(layers, std::max<int64_t>(1, hz / (static_cast<int64_t>(rows_per) * row_layer))));
   const int nsm = host::sm_count();
-  const bool small = chunk_items(page_size) == CH_SMALL;   // matches the kernels' copy path
+  const bool small = chunk_items(slice) == CH_SMALL;   // matches the kernels' copy path
   for (int r0 = 0; r0 < num_rows; r0 += rows_per) {
     const int nr = std::min(rows_per, num_rows - r0);
     for (int l0 = 0; l0 < layers; l0 += group) {
@@ -2703,6 +2726,59 @@ extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_w
     if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("bzero_kernel");
   }
   return CE_OK;
+}
+}  // namespace
+
+extern "C" int ce_boundary(int32_t* table, int64_t table_stride, int32_t table_width,
+                           int32_t* req_to_unit, int64_t r2u_stride, int32_t r2u_width,
+                           int32_t* frontier, int32_t* count, int32_t* pos,
+                           int64_t pos_row_stride, int32_t pos_cap, float* scores,
+                           int64_t score_layer_stride, int64_t score_head_stride,
+                           int64_t pool_units, const uint64_t* k_layers,
+                           const uint64_t* v_layers, int32_t layers, int32_t kv_heads,
+                           int32_t head_dim, int32_t page_size, int32_t head_offset,
+                           int32_t* marks, int32_t epoch, const int64_t* swa_mapping,
+                           const int32_t* rows, const ce_row_params* params, int32_t num_rows,
+                           const void* uniforms, int32_t uniform_dtype,
+                           const float* global_scores, int32_t global_heads, int32_t live,
+                           int32_t max_cols, int32_t max_width, int32_t max_n, int32_t* result,
+                           int32_t* freed_units, int64_t freed_stride, void* workspace,
+                           int64_t workspace_bytes, int64_t hazard_bytes, uint32_t* record_delta,
+                           int64_t record_stride, int32_t* record_counts, int32_t* err,
+                           void* stream) {
+  return boundary_call(false, table, table_stride, table_width, req_to_unit, r2u_stride, r2u_width, frontier,
+                       count, pos, pos_row_stride, pos_cap, scores, score_layer_stride, score_head_stride,
+                       pool_units, k_layers, v_layers, layers, kv_heads, head_dim, page_size, head_offset,
+                       marks, epoch, swa_mapping, rows, params, num_rows, uniforms, uniform_dtype,
+                       global_scores, global_heads, live, max_cols, max_width, max_n, result, freed_units,
+                       freed_stride, workspace, workspace_bytes, hazard_bytes, record_delta, record_stride,
+                       record_counts, err, stream);
+}
+
+extern "C" int ce_kv4_boundary(int32_t* table, int64_t table_stride, int32_t table_width,
+                               int32_t* req_to_unit, int64_t r2u_stride, int32_t r2u_width,
+                               int32_t* frontier, int32_t* count, int32_t* pos,
+                               int64_t pos_row_stride, int32_t pos_cap, float* scores,
+                               int64_t score_layer_stride, int64_t score_head_stride,
+                               int64_t pool_units, const uint64_t* k_layers,
+                               const uint64_t* v_layers, int32_t layers, int32_t kv_heads,
+                               int32_t head_dim, int32_t page_size, int32_t head_offset,
+                               int32_t* marks, int32_t epoch, const int64_t* swa_mapping,
+                               const int32_t* rows, const ce_row_params* params, int32_t num_rows,
+                               const void* uniforms, int32_t uniform_dtype,
+                               const float* global_scores, int32_t global_heads, int32_t live,
+                               int32_t max_cols, int32_t max_width, int32_t max_n, int32_t* result,
+                               int32_t* freed_units, int64_t freed_stride, void* workspace,
+                               int64_t workspace_bytes, int64_t hazard_bytes, uint32_t* record_delta,
+                               int64_t record_stride, int32_t* record_counts, int32_t* err,
+                               void* stream) {
+  return boundary_call(true, table, table_stride, table_width, req_to_unit, r2u_stride, r2u_width, frontier,
+                       count, pos, pos_row_stride, pos_cap, scores, score_layer_stride, score_head_stride,
+                       pool_units, k_layers, v_layers, layers, kv_heads, head_dim, page_size, head_offset,
+                       marks, epoch, swa_mapping, rows, params, num_rows, uniforms, uniform_dtype,
+                       global_scores, global_heads, live, max_cols, max_width, max_n, result, freed_units,
+                       freed_stride, workspace, workspace_bytes, hazard_bytes, record_delta, record_stride,
+                       record_counts, err, stream);
 }
 
 extern "C" int ce_reservoir_scores(const int32_t* pos, int32_t layers, int32_t heads, int32_t n_cols,

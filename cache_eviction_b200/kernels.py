@@ -187,6 +187,203 @@ def decode_scores(kv_indptr, kv_indices, kv_tokens, pool_units, page_size, H, G,
     _count(1 if score_flags & 3 else 0)
 
 
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on(device: torch.device, *tensors) -> None:
+    """Every tensor given lies on `device` (a CUDA device)."""
+    _require(device.type == "cuda" and all(t is None or t.device == device for t in tensors),
+             f"every tensor must be on one CUDA device, here {device}")
+
+
+def _csr(kv_indptr, kv_indices, kv_tokens, bs: int) -> None:
+    for t in (kv_indptr, kv_indices, kv_tokens):
+        _require(t.dtype == torch.int32 and t.is_contiguous(), "kv_indptr, kv_indices and kv_tokens must be dense int32")
+    _require(kv_indptr.numel() >= bs + 1 and kv_tokens.numel() >= bs, "kv_indptr or kv_tokens shorter than the batch")
+
+
+def _sinks(sinks, H: int):
+    if sinks is None:
+        return None
+    _require(sinks.numel() == H, "sinks must hold one value per query head")
+    return sinks.to(torch.float32).contiguous()
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t [.., 64] with 16-byte aligned rows: itself, or a dense copy."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(st % 8 == 0 for st in t.stride()[:-1]):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _workspace(need: int, given: Optional[torch.Tensor], device, what: str) -> torch.Tensor:
+    """The caller's workspace, or one from torch's allocator for this call
+    alone, which is safe on any stream and inside a capture (a graph keeps it)."""
+    if need < 0:
+        raise capi.CeError(f"{what} failed")
+    if given is None:
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    _require(given.dtype == torch.uint8 and given.is_contiguous() and given.numel() >= need and given.device == device,
+             f"workspace must be a dense uint8 tensor of at least {need} bytes on {device}")
+    return given
+
+
+def kv4_pool(units: int, kv_heads: int, device) -> torch.Tensor:
+    """An empty pool of 4-bit pages of 16 tokens (one layer's K or V)."""
+    return torch.empty((units, kv_heads, capi.CE_KV4_SLICE_BYTES), dtype=torch.uint8, device=device)
+
+
+def _kv4_pools(k_pool, v_pool):
+    for t in (k_pool, v_pool):
+        _require(t.dtype == torch.uint8 and t.dim() == 3 and t.is_contiguous() and t.shape == k_pool.shape
+                 and t.shape[2] == capi.CE_KV4_SLICE_BYTES,
+                 f"4-bit pools must be dense uint8 [units, kv_heads, {capi.CE_KV4_SLICE_BYTES}] of one shape")
+    return k_pool.shape[0], k_pool.shape[1]
+
+
+def kv4_write(k, v, k_pool, v_pool, loc, err=None):
+    """Quantise K and V rows to 4 bits into their slots (ce_kv4_write).
+
+    k, v [tokens, G, 64] bf16 (any strides; rows that are not 16-byte aligned
+    are copied first); pools from kv4_pool; loc [tokens] int64 slots, unit * 16
+    + position in the page, distinct, negative ones skipped."""
+    lib = capi.load()
+    units, G = _kv4_pools(k_pool, v_pool)
+    _require(k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.dim() == 3 and k.shape == v.shape
+             and tuple(k.shape[1:]) == (G, 64), f"k and v must be bf16 [tokens, {G}, 64]")
+    _require(loc.dtype == torch.int64 and loc.is_contiguous() and loc.numel() == k.shape[0],
+             "loc must hold one int64 slot per token")
+    _on(k_pool.device, k, v, v_pool, loc, err)
+    k, v = _rows16(k), _rows16(v)
+    with torch.cuda.device(k_pool.device):
+        st = lib.ce_kv4_write(_p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(loc), k.shape[0], G,
+                              64, 16, _p(k_pool), _p(v_pool), units, _p(err), _stream(k_pool.device))
+    capi.check(st, "ce_kv4_write")
+    _count(1 if k.shape[0] else 0)
+
+
+def kv4_read(k_pool, v_pool, units, k_out=None, v_out=None, err=None):
+    """Pages `units` [n] int32 of 4-bit pools as bf16 (ce_kv4_read): k_out and
+    v_out [n, G, 16, 64], allocated unless given (any strides with 16-byte
+    aligned rows).  Pages of negative units are left as they are."""
+    lib = capi.load()
+    pool_units, G = _kv4_pools(k_pool, v_pool)
+    _require(units.dtype == torch.int32 and units.dim() == 1 and units.is_contiguous(), "units must be dense int32 [n]")
+    n = int(units.numel())
+    shape = (n, G, 16, 64)
+    k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pool.device) if k_out is None else k_out
+    v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pool.device) if v_out is None else v_out
+    for t in (k_out, v_out):
+        _require(t.dtype == torch.bfloat16 and tuple(t.shape) == shape and (n == 0 or t.stride(3) == 1),
+                 f"outputs must be bf16 {list(shape)} with dense rows")
+    _on(k_pool.device, v_pool, units, k_out, v_out, err)
+    with torch.cuda.device(k_pool.device):
+        st = lib.ce_kv4_read(_p(k_pool), _p(v_pool), pool_units, _p(units), n, G, 64, 16, _p(k_out), *k_out.stride()[:3],
+                             _p(v_out), *v_out.stride()[:3], _p(err), _stream(k_pool.device))
+    capi.check(st, "ce_kv4_read")
+    _count(1 if n else 0)
+    return k_out, v_out
+
+
+def kv4_decode_workspace_bytes(bs, kv_capacity, H, G, score_flags=3):
+    need = capi.load().ce_kv4_decode_workspace_bytes(bs, kv_capacity, H, G, score_flags)
+    if need < 0:
+        raise capi.CeError("ce_kv4_decode_workspace_bytes failed")
+    return need
+
+
+def kv4_decode_attn_score(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sm_scale, sinks=None,
+                          mode_of_row=None, rows=None, scores=None, zero_new=True, out=None, lse=None,
+                          score_flags=3, err=None, workspace=None):
+    """Fused decode attention + H2O score over one layer's 4-bit pages
+    (ce_kv4_decode_attn_score): decode_attn_score with pools from kv4_pool,
+    16-token pages and a bf16 output.  capi.CE_SCORE_DEFER in score_flags
+    leaves the page scores to decode_scores, from the workspace then given."""
+    lib = capi.load()
+    units, G = _kv4_pools(k_pool, v_pool)
+    _require(q.dim() == 3 and q.dtype == torch.bfloat16, "q must be bf16 [batch, query heads, 64]")
+    bs, H, D = q.shape
+    dev = q.device
+    _csr(kv_indptr, kv_indices, kv_tokens, bs)
+    if q.numel() and (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 2 or q.data_ptr() % 4):
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty((bs, H, D), dtype=torch.bfloat16, device=dev) if out is None else out
+    _require(out.dtype == torch.bfloat16 and tuple(out.shape) == (bs, H, D) and (bs == 0 or out.stride(2) == 1),
+             "out must be bf16 of q's shape with dense rows")
+    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == bs * H),
+             "lse must be dense fp32 [batch, query heads]")
+    if scores is not None:
+        _require(scores.dtype == torch.float32 and scores.dim() == 2 and scores.shape[0] == G
+                 and scores.shape[1] >= units and scores.stride(1) == 1, "scores must be fp32 [kv_heads, units]")
+    _require(mode_of_row is None or (mode_of_row.dtype == torch.int32 and mode_of_row.is_contiguous()),
+             "mode_of_row must be dense int32")
+    _require(rows is None or (rows.dtype == torch.int64 and rows.is_contiguous() and rows.numel() >= bs),
+             "rows must hold one int64 row per batch entry")
+    _require(mode_of_row is None or rows is not None or mode_of_row.numel() >= bs, "mode_of_row shorter than the batch")
+    _require(workspace is not None or not score_flags & capi.CE_SCORE_DEFER,
+             "deferred scores need the caller's workspace")
+    _on(dev, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, mode_of_row, rows, scores, out, lse, err)
+    sinks = _sinks(sinks, H)
+    cap = kv_indices.numel()
+    with torch.cuda.device(dev):
+        ws = _workspace(lib.ce_kv4_decode_workspace_bytes(bs, cap, H, G, score_flags), workspace, dev,
+                        "ce_kv4_decode_workspace_bytes")
+        st = lib.ce_kv4_decode_attn_score(
+            _p(q), q.stride(0), q.stride(1), _p(k_pool), _p(v_pool), units, _p(kv_indptr), _p(kv_indices),
+            _p(kv_tokens), cap, _p(sinks), _p(mode_of_row), _p(rows), float(sm_scale), bs, H, G, D, 16, _p(scores),
+            scores.stride(0) if scores is not None else 0, 1 if zero_new else 0, _p(out), out.stride(0), out.stride(1),
+            _p(lse), score_flags, _p(ws), ws.numel(), _p(err), _stream(dev))
+    capi.check(st, "ce_kv4_decode_attn_score")
+    _count(2 if bs else 0)
+    return out
+
+
+def _bf16_pools(k_pool, v_pool, page_size):
+    for t in (k_pool, v_pool):
+        _require(t.dtype == torch.bfloat16 and t.dim() == 4 and t.is_contiguous() and t.shape == k_pool.shape
+                 and tuple(t.shape[2:]) == (page_size, 64), f"pools must be dense bf16 [units, kv_heads, {page_size}, 64]")
+    return k_pool.shape[0], k_pool.shape[1]
+
+
+def window_decode(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sm_scale, page_size, window, first=0,
+                  sinks=None, out=None, out_f32=False, lse=None, err=None, workspace=None):
+    """One token per sequence attending to the last `window` tokens (itself
+    among them; -1: all) and to its first `first` tokens (ce_window_decode).
+
+    q [bs, H, 64] bf16; pools [units, G, page, 64] bf16; the CSR of fill().
+    Returns out [bs, H, 64] (bf16, or fp32 with out_f32)."""
+    lib = capi.load()
+    units, G = _bf16_pools(k_pool, v_pool, page_size)
+    _require(q.dim() == 3 and q.dtype == torch.bfloat16, "q must be bf16 [batch, query heads, 64]")
+    bs, H, D = q.shape
+    dev = q.device
+    _csr(kv_indptr, kv_indices, kv_tokens, bs)
+    if q.numel() and (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 2 or q.data_ptr() % 4):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((bs, H, D), dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
+    _require(out.dtype in (torch.float32, torch.bfloat16) and tuple(out.shape) == (bs, H, D)
+             and (bs == 0 or out.stride(2) == 1), "out must be bf16 or fp32 of q's shape with dense rows")
+    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == bs * H),
+             "lse must be dense fp32 [batch, query heads]")
+    _on(dev, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, out, lse, err)
+    sinks = _sinks(sinks, H)
+    cap = kv_indices.numel()
+    with torch.cuda.device(dev):
+        ws = _workspace(lib.ce_decode_workspace_bytes(bs, cap, H, G, page_size, 0), workspace, dev,
+                        "ce_decode_workspace_bytes")
+        st = lib.ce_window_decode(
+            _p(q), q.stride(0), q.stride(1), _p(k_pool), _p(v_pool), units, _p(kv_indptr), _p(kv_indices),
+            _p(kv_tokens), cap, _p(sinks), float(sm_scale), bs, H, G, D, page_size, int(window), int(first), _p(out),
+            1 if out.dtype == torch.float32 else 0, out.stride(0), out.stride(1), _p(lse), _p(ws), ws.numel(), _p(err),
+            _stream(dev))
+    capi.check(st, "ce_window_decode")
+    _count(2 if bs else 0)
+    return out
+
+
 def prefill_scores(q, k_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sm_scale, page_size,
                    max_q, max_tokens, sinks=None, mode_of_row=None, rows=None, scores=None,
                    zero_new=True, err=None):

@@ -452,6 +452,113 @@ int ce_reservoir_scores(const int32_t* pos, int32_t layers, int32_t heads,
                         int32_t n_cols, int32_t head_offset, uint64_t seed,
                         uint64_t* out, void* stream);
 
+/* ---- 4-bit KV cache ---------------------------------------------------------
+ * No counterpart in the reference.  A pool of 4-bit pages takes the place of
+ * a layer's bf16 pool of 16-token pages: [pool_units, G] slices of
+ * CE_KV4_SLICE_BYTES (576 instead of 2,048) bytes, 16-byte aligned.  Of each
+ * (token, KV head) row x of 64 values it keeps
+ *   m = min(x), s = bf16((max / 2 - min / 2) * (2 / 15)),
+ *   c = clamp(rint((x - m) / s), 0, 15)   (fp32, ties to even; 0 where s = 0)
+ * and a value is m + c * s.  A row with a NaN or an infinity reads as NaN
+ * throughout.  Bytes 0..511 of a slice hold the codes, bytes 512 + 4 j the
+ * scale and then the minimum (bf16) of token j:
+ *   K  dims 16 t .. 16 t + 15 of token j are the 8 bytes at
+ *      ((j / 2) * 4 + t) * 16 + (j % 2) * 8, an even dim in a byte's low half;
+ *   V  byte ((j / 4) * 8 + r) * 16 + q * 4 + j % 4 holds dims 16 q + r (low
+ *      half) and 16 q + r + 8 of token j.
+ * Supported: head_dim 64, 16-token pages.
+ *
+ * ce_kv4_write: K and V rows of `tokens` tokens into their slots.
+ *   k, v    [tokens, G, 64] bf16 (token and head strides k_st, k_sg, v_st,
+ *           v_sg in elements, multiples of 8; last dim dense; 16-byte aligned)
+ *   loc     [tokens] token slots, unit * 16 + position in the page; a negative
+ *           one skips the token (padding), one beyond the pool flags
+ *           CE_EW_INDEX and skips it.  Slots must differ: of two tokens given
+ *           the same slot in one call it holds a mixture. */
+#define CE_KV4_SLICE_BYTES 576
+int ce_kv4_write(const void* k, int64_t k_st, int64_t k_sg, const void* v, int64_t v_st, int64_t v_sg,
+                 const int64_t* loc, int64_t tokens, int32_t num_kv_heads, int32_t head_dim,
+                 int32_t page_size, void* k_pool, void* v_pool, int64_t pool_units,
+                 int32_t* err, void* stream);
+
+/* ce_kv4_read: pages units[0 .. num_units) as bf16, page i, head g, position j
+ * to out + i * ou + g * og + j * ot (elements, multiples of 8; 64 dense
+ * values, 16-byte aligned): [num_units, G, 16, 64] is a bf16 pool whose unit i
+ * is the i-th page listed, for ce_prefill_scores.  A
+ * negative unit skips its page (the output keeps what it held), one beyond
+ * the pool flags CE_EW_INDEX and skips it. */
+int ce_kv4_read(const void* k_pool, const void* v_pool, int64_t pool_units, const int32_t* units,
+                int64_t num_units, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                void* k_out, int64_t k_ou, int64_t k_og, int64_t k_ot,
+                void* v_out, int64_t v_ou, int64_t v_og, int64_t v_ot,
+                int32_t* err, void* stream);
+
+/* ce_kv4_decode_attn_score: ce_decode_attn_score over pools of 4-bit pages.
+ * Arguments, scores and score_flags (CE_SCORE_DEFER too, with
+ * ce_decode_scores afterwards) as there, except that kv_tokens is required,
+ * the output is bf16, sm_scale is positive and score_sg >= pool_units.  Slots
+ * beyond a row's tokens may hold anything.
+ * Supported: head_dim 64, H/G == 8, G 1, 2, 4 or 8, page_size 16. */
+int64_t ce_kv4_decode_workspace_bytes(int32_t bs, int64_t kv_capacity, int32_t num_q_heads,
+                                      int32_t num_kv_heads, int32_t score_flags);
+int ce_kv4_decode_attn_score(const void* q, int64_t q_sb, int64_t q_sh,
+                             const void* k_pool, const void* v_pool, int64_t pool_units,
+                             const int32_t* kv_indptr, const int32_t* kv_indices,
+                             const int32_t* kv_tokens, int64_t kv_capacity,
+                             const float* sinks, const int32_t* mode_of_row, const int64_t* rows,
+                             float sm_scale, int32_t bs, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                             float* scores, int64_t score_sg, int32_t zero_new,
+                             void* out, int64_t o_sb, int64_t o_sh, float* lse_out,
+                             int32_t score_flags, void* workspace, int64_t workspace_bytes,
+                             int32_t* err, void* stream);
+
+/* ce_kv4_boundary: ce_boundary over pools of 4-bit pages (k_layers and
+ * v_layers hold their addresses, page_size is 16).  Pages move as they are,
+ * without being requantised. */
+int64_t ce_kv4_boundary_workspace_bytes(int32_t num_rows, int32_t layers, int32_t kv_heads,
+                                        int32_t head_dim, int32_t page_size, int32_t max_cols,
+                                        int32_t max_width, int64_t hazard_bytes);
+int ce_kv4_boundary(int32_t* table, int64_t table_stride, int32_t table_width,
+                    int32_t* req_to_unit, int64_t r2u_stride, int32_t r2u_width,
+                    int32_t* frontier, int32_t* count,
+                    int32_t* pos, int64_t pos_row_stride, int32_t pos_cap,
+                    float* scores, int64_t score_layer_stride, int64_t score_head_stride,
+                    int64_t pool_units,
+                    const uint64_t* k_layers, const uint64_t* v_layers,
+                    int32_t layers, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                    int32_t head_offset,
+                    int32_t* marks, int32_t epoch, const int64_t* swa_mapping,
+                    const int32_t* rows, const ce_row_params* params, int32_t num_rows,
+                    const void* uniforms, int32_t uniform_dtype,
+                    const float* global_scores, int32_t global_heads,
+                    int32_t live, int32_t max_cols, int32_t max_width, int32_t max_n,
+                    int32_t* result, int32_t* freed_units, int64_t freed_stride,
+                    void* workspace, int64_t workspace_bytes, int64_t hazard_bytes,
+                    uint32_t* record_delta, int64_t record_stride, int32_t* record_counts,
+                    int32_t* err, void* stream);
+
+/* ---- windowed attention -----------------------------------------------------
+ * Attention to a sliding window and to a few first tokens that stay visible,
+ * over the paged bf16 pools and CSR lists of ce_decode_attn_score (outputs
+ * only).  A query at list position p sees list token t iff
+ *   t <= p and (t > p - window or t < first),      window >= 1,
+ * or t <= p alone when window is -1.  No counterpart in the reference (SGLang
+ * runs its sliding-window layers itself).
+ *
+ * ce_window_decode: one query per entry, at position kv_tokens[b] - 1 (an
+ * entry without tokens gets zeros).  q, pools, CSR, sinks, out, lse_out and
+ * the workspace (ce_decode_workspace_bytes with score_flags 0) as for
+ * ce_decode_attn_score, kv_tokens required.  Only pages with a visible token
+ * are read; what the others' slots hold does not matter. */
+int ce_window_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool, const void* v_pool,
+                     int64_t pool_units, const int32_t* kv_indptr, const int32_t* kv_indices,
+                     const int32_t* kv_tokens, int64_t kv_capacity, const float* sinks, float sm_scale,
+                     int32_t bs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t page_size, int32_t window, int32_t first, void* out, int32_t out_f32,
+                     int64_t o_sb, int64_t o_sh, float* lse_out, void* workspace,
+                     int64_t workspace_bytes, int32_t* err, void* stream);
+
 /* ---- self-test of the bounded device waits --------------------------------
  * Every pipelined kernel waits on mbarrier phases with a bound (2 s): a wait
  * that runs out flags CE_EW_TIMEOUT, tells the CTA's other warps to stop and

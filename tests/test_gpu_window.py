@@ -1,0 +1,162 @@
+"""Windowed attention on the GPU (ce_window_decode, ce_window_prefill) against
+the same mask in 64 bits.
+
+Tolerances per value, from the arithmetic: logits are fp32 sums of 64 exact
+bf16 products, off by at most d = 80 * 2^-24 * scale * sum |q k|; a p is off by
+at most the relative e = 2 d + 16 * 2^-24 * (1 + |logit range|).  The decode form
+splits p into two bf16 parts (2^-17), so |error| <= (2^-17 + e) sum p |v| plus the
+output's rounding (2^-8 in bf16, 2^-24 in fp32).  The prefill form rounds p to
+bf16 (2^-8 of each) and takes a share of its exponentials from a polynomial
+(2^-13, coefficients' fit 7.6e-5): |error| <= (2^-8 + 2^-12 + e) sum p |v| + 2^-8 |o|.
+"""
+import math
+
+import pytest
+import torch
+
+import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+SCALE = 0.125
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from cache_eviction_b200 import capi
+    capi.load()
+
+
+def batch(lens, G, P, gen, garbage=float("nan")):
+    """Scattered bf16 pages of a batch; every slot that holds no token of a row
+    holds `garbage`."""
+    counts = [-(-n // P) for n in lens]
+    units = sum(counts) + 3
+    order = torch.randperm(units, generator=gen)[:sum(counts)]
+    indptr = torch.tensor([0] + counts).cumsum(0)
+    pools = torch.full((2, units, G, P, 64), garbage, dtype=torch.bfloat16)
+    flat = []
+    for b, n in enumerate(lens):
+        x = (torch.randn((2, n, G, 64), generator=gen) + 0.3 * torch.randn((2, 1, G, 64), generator=gen)).to(torch.bfloat16)
+        flat.append(x)
+        t = torch.arange(n)
+        u = order[indptr[b] + t // P]
+        pools[:, u, :, t % P] = x.transpose(0, 1)
+    csr = (indptr.to(torch.int32).to(DEV), order.to(torch.int32).to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    return pools, flat, csr, order, indptr
+
+
+def visible(pos, n, window, first):
+    """[len(pos), n] mask of the definition."""
+    t = torch.arange(n)[None]
+    m = t <= pos[:, None]
+    return m & ((t > pos[:, None] - window) | (t < first)) if window >= 0 else m
+
+
+def hold(got, q, k, v, seen, sink, bf16_p, lse=None, f32=False):
+    """got [n, 8, 64] of one KV head against the 64-bit form."""
+    if k.shape[0] == 0:      # nothing but the sink
+        assert (got == 0).all()
+        want = torch.full((8,), -math.inf) if sink is None else sink
+        assert lse is None or torch.allclose(lse.double()[0], want.double(), rtol=2.0 ** -22, atol=2.0 ** -22)
+        return
+    q, k, v = q.double(), k.double(), v.double()
+    p, o, l = ref.attend(q, k, v, seen, sink, SCALE)
+    d = 80 * 2.0 ** -24 * SCALE * torch.einsum("njd,td->njt", q.abs(), k.abs())
+    d = torch.where(seen[:, None], d, 0.0).amax(-1)
+    z = torch.einsum("njd,td->njt", q, k) * SCALE
+    span = torch.where(seen[:, None], (z - l[..., None]).abs(), 0.0).amax(-1)
+    e = 2 * d + 16 * 2.0 ** -24 * (1 + span)
+    e = torch.where(l.isinf(), 0.0, e)[..., None]
+    w = 2.0 ** -8 + 2.0 ** -12 if bf16_p else 2.0 ** -17
+    tol = (w + e) * torch.einsum("njt,td->njd", p, v.abs()) + (2.0 ** -24 if f32 else 2.0 ** -8) * o.abs() + 1e-30
+    bad = ((got.double() - o).abs() / tol)
+    assert not got.isnan().any() and (bad <= 1).all(), float(bad.nan_to_num(1e9).max())
+    if lse is not None:
+        ok = torch.where(l.isinf(), lse.double() == l, (lse.double() - l).abs() <= e[..., 0] + 2.0 ** -22 * (1 + l.abs()))
+        assert ok.all()
+
+
+# ------------------------------------------------------------ single tokens
+def check_step(lens, G, P, window, first, seed, sinks=True, call=None, **kw):
+    from cache_eviction_b200 import kernels
+    gen = torch.Generator().manual_seed(seed)
+    B, H = len(lens), 8 * G
+    pools, flat, csr, order, indptr = batch(lens, G, P, gen)
+    if window >= 0:     # what the mask hides may hold anything, in pages that are partly visible too
+        for b, n in enumerate(lens):
+            t = torch.arange(n)
+            t = t[~visible(torch.tensor([n - 1]), n, window, first)[0]]
+            bad = torch.tensor([math.nan, math.inf, -math.inf, -3.3895e38])[t % 4].to(torch.bfloat16)
+            pools[:, order[indptr[b] + t // P], :, t % P] = bad.view(-1, 1, 1, 1)
+    q = (torch.randn((B, H, 64), generator=gen) * 1.5).to(torch.bfloat16)
+    sink = torch.randn(H, generator=gen) if sinks else None
+    err, lse = torch.zeros(1, dtype=torch.int32, device=DEV), torch.empty((B, H), device=DEV)
+    out = (call or kernels.window_decode)(q.to(DEV), pools[0].to(DEV), pools[1].to(DEV), *csr, SCALE, P, window, first=first,
+                                          sinks=None if sink is None else sink.to(DEV), lse=lse, err=err, **kw)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    for b, n in enumerate(lens):
+        seen = visible(torch.tensor([n - 1]), n, window, first)
+        for g in range(G):
+            hs = slice(8 * g, 8 * g + 8)
+            hold(out[b:b + 1, hs].cpu(), q[b:b + 1, hs], flat[b][0][:, g], flat[b][1][:, g], seen,
+                 None if sink is None else sink[hs].double(), False, lse[b:b + 1, hs].cpu(), out.dtype == torch.float32)
+    return out
+
+
+LENS = [1, 2, 15, 16, 17, 31, 100, 127, 128, 129, 0, 255, 257, 511, 700, 1000, 0]
+
+
+@pytest.mark.parametrize("G,P", [(1, 16), (2, 16), (4, 16), (8, 16), (8, 1)])
+@pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (16, 0), (17, 3), (128, 0), (100, 16), (130, 129), (513, 40),
+                                          (1, 600), (2 ** 31 - 1, 2 ** 31 - 1), (-1, 0), (-1, 5)])
+def test_step_masks(G, P, window, first):
+    check_step(LENS, G, P, window, first, seed=G + P + window % 97)
+
+
+@pytest.mark.parametrize("n,window,first", [(20011, 4099, 5), (20011, 6000, 2048), (50000, 128, 0), (1, 1, 0)])
+def test_step_one_sequence(n, window, first):
+    check_step([n], 8, 16, window, first, seed=n)
+    check_step([n], 1, 16, window, first, seed=n, sinks=False, out_f32=True)
+
+
+def test_step_without_a_window_is_the_plain_decode():
+    from cache_eviction_b200 import kernels
+    gen = torch.Generator().manual_seed(3)
+    pools, _, csr, _, _ = batch([300, 17, 2000, 0, 64], 4, 16, gen)
+    q = torch.randn((5, 32, 64), generator=gen).to(torch.bfloat16).to(DEV)
+    a = (q, pools[0].to(DEV), pools[1].to(DEV), *csr, SCALE, 16)
+    want = kernels.decode_attn_score(*a, score_flags=0)
+    for window, first in ((-1, 0), (2000, 0), (5000, 7), (1, 5000)):
+        assert torch.equal(kernels.window_decode(*a, window, first=first), want)
+
+
+def test_step_strides_stream_and_graph():
+    from cache_eviction_b200 import kernels
+    side = torch.cuda.Stream()
+    wide = torch.zeros((3, 70, 192), dtype=torch.bfloat16, device=DEV)
+
+    def strided(q, *a, **kw):
+        view = torch.zeros((3, 65, 131), dtype=torch.bfloat16, device=DEV)[:, 1:, 3:67]     # odd strides: copied
+        view.copy_(q)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = kernels.window_decode(view, *a, out=wide[:, 3:67, 64:128], **kw)
+        torch.cuda.current_stream().wait_stream(side)
+        return out
+
+    def captured(q, *a, **kw):
+        kernels.window_decode(q, *a, **kw)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = kernels.window_decode(q, *a, **kw)
+        out.zero_()
+        graph.replay()
+        return out
+    a = check_step([300, 17, 1025], 8, 16, 200, 20, seed=10, call=strided)
+    b = check_step([300, 17, 1025], 8, 16, 200, 20, seed=10, call=captured)
+    assert torch.equal(a, b)
+    assert (wide[:, :3] == 0).all() and (wide[:, :, :64] == 0).all() and (wide[:, :, 128:] == 0).all()
