@@ -384,6 +384,41 @@ def window_decode(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sm_scale,
     return out
 
 
+def window_prefill(q, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sm_scale, page_size, max_q,
+                   max_tokens, window, first=0, sinks=None, out=None, err=None):
+    """Causal attention of extend chunks with a sliding window and first tokens
+    (ce_window_prefill): q [total_q, H, 64] bf16, entry b's chunk being rows
+    qo_indptr[b] .. qo_indptr[b+1] at the end of its kv_tokens[b] list tokens;
+    max_q / max_tokens bound the chunk and list lengths (host ints).  Returns
+    out [total_q, H, 64] bf16; rows of no entry keep what they held."""
+    lib = capi.load()
+    units, G = _bf16_pools(k_pool, v_pool, page_size)
+    _require(q.dim() == 3 and q.dtype == torch.bfloat16, "q must be bf16 [queries, query heads, 64]")
+    total_q, H, D = q.shape
+    bs = int(kv_tokens.numel())
+    dev = q.device
+    _csr(kv_indptr, kv_indices, kv_tokens, bs)
+    _require(qo_indptr.dtype == torch.int32 and qo_indptr.is_contiguous() and qo_indptr.numel() >= bs + 1,
+             "qo_indptr must hold one more dense int32 than there are entries")
+    if q.numel() and (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16
+                      or q.stride(1) < D or q.stride(0) < H * q.stride(1)):
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty((total_q, H, D), dtype=torch.bfloat16, device=dev) if out is None else out
+    _require(out.dtype == torch.bfloat16 and tuple(out.shape) == (total_q, H, D) and (total_q == 0 or out.stride(2) == 1),
+             "out must be bf16 of q's shape with dense rows")
+    _on(dev, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sinks, out, err)
+    sinks = _sinks(sinks, H)
+    with torch.cuda.device(dev):
+        st = lib.ce_window_prefill(
+            _p(q), q.stride(0), q.stride(1), _p(k_pool), _p(v_pool), units, _p(qo_indptr), _p(kv_indptr),
+            _p(kv_indices), _p(kv_tokens), kv_indices.numel(), _p(sinks), float(sm_scale), bs, H, G, D, page_size,
+            total_q, int(max_q), int(max_tokens), int(window), int(first), _p(out), out.stride(0), out.stride(1),
+            _p(err), _stream(dev))
+    capi.check(st, "ce_window_prefill")
+    _count(1 if bs and max_q and total_q else 0)
+    return out
+
+
 def prefill_scores(q, k_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sm_scale, page_size,
                    max_q, max_tokens, sinks=None, mode_of_row=None, rows=None, scores=None,
                    zero_new=True, err=None):

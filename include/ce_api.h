@@ -484,7 +484,7 @@ int ce_kv4_write(const void* k, int64_t k_st, int64_t k_sg, const void* v, int64
 /* ce_kv4_read: pages units[0 .. num_units) as bf16, page i, head g, position j
  * to out + i * ou + g * og + j * ot (elements, multiples of 8; 64 dense
  * values, 16-byte aligned): [num_units, G, 16, 64] is a bf16 pool whose unit i
- * is the i-th page listed, for ce_prefill_scores.  A
+ * is the i-th page listed, for ce_prefill_scores and ce_window_prefill.  A
  * negative unit skips its page (the output keeps what it held), one beyond
  * the pool flags CE_EW_INDEX and skips it. */
 int ce_kv4_read(const void* k_pool, const void* v_pool, int64_t pool_units, const int32_t* units,
@@ -558,6 +558,23 @@ int ce_window_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k_po
                      int32_t page_size, int32_t window, int32_t first, void* out, int32_t out_f32,
                      int64_t o_sb, int64_t o_sh, float* lse_out, void* workspace,
                      int64_t workspace_bytes, int32_t* err, void* stream);
+
+/* ce_window_prefill: the queries of a ragged batch of extend chunks, entry
+ * b's being rows qo_indptr[b] .. qo_indptr[b+1] of q at the last list
+ * positions of its kv_tokens[b] tokens (q, CSR, max_q and max_tokens as for
+ * ce_prefill_scores).  out [total_q, H, 64] bf16 (strides o_st, o_sh, multiples
+ * of 8; 16-byte aligned); rows of no entry keep what they held.  An entry
+ * whose ranges do not fit flags CE_EW_SHAPE and keeps its rows.  A visible
+ * value that is not finite makes its rows' outputs NaN (or infinite); what a
+ * row does not see does not reach it.
+ * Supported: head_dim 64, H == 8*G, page_size dividing 64, sm_scale > 0. */
+int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, const void* k_pool, const void* v_pool,
+                      int64_t pool_units, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                      const int32_t* kv_indices, const int32_t* kv_tokens, int64_t kv_capacity,
+                      const float* sinks, float sm_scale, int32_t bs, int32_t num_q_heads,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t total_q,
+                      int32_t max_q, int32_t max_tokens, int32_t window, int32_t first,
+                      void* out, int64_t o_st, int64_t o_sh, int32_t* err, void* stream);
 
 /* ---- self-test of the bounded device waits --------------------------------
  * Every pipelined kernel waits on mbarrier phases with a bound (2 s): a wait

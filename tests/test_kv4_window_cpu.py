@@ -65,6 +65,16 @@ REFUSALS = [
     ("ce_window_decode", dict(num_q_heads=56), UNSUPPORTED), ("ce_window_decode", dict(page_size=8), UNSUPPORTED),
     ("ce_window_decode", dict(page_size=1, num_q_heads=32, num_kv_heads=4), UNSUPPORTED),
     ("ce_window_decode", dict(head_dim=80), UNSUPPORTED), ("ce_window_decode", dict(q_sh=63), ARG),
+    ("ce_window_prefill", dict(window=0), ARG), ("ce_window_prefill", dict(window=-3), ARG),
+    ("ce_window_prefill", dict(first=-1), ARG), ("ce_window_prefill", dict(sm_scale=0.0), ARG),
+    ("ce_window_prefill", dict(total_q=-1), ARG), ("ce_window_prefill", dict(max_tokens=-1), ARG),
+    ("ce_window_prefill", dict(max_tokens=2 ** 31 - 1), UNSUPPORTED), ("ce_window_prefill", dict(bs=65536), UNSUPPORTED),
+    ("ce_window_prefill", dict(head_dim=128), UNSUPPORTED), ("ce_window_prefill", dict(num_q_heads=8), UNSUPPORTED),
+    ("ce_window_prefill", dict(page_size=128), UNSUPPORTED), ("ce_window_prefill", dict(page_size=24), UNSUPPORTED),
+    ("ce_window_prefill", dict(pool_units=1 << 26), UNSUPPORTED), ("ce_window_prefill", dict(pool_units=0), ARG),
+    ("ce_window_prefill", dict(q_st=2048), ARG), ("ce_window_prefill", dict(q_sh=68), ARG),
+    ("ce_window_prefill", dict(o_st=4100), ARG), ("ce_window_prefill", dict(out=4104), ARG),
+    ("ce_window_prefill", dict(v_pool=4100), ARG),
 ]
 
 
@@ -78,7 +88,8 @@ def test_refused_on_the_host(name, values, want):
     ("ce_kv4_write", ["k", "v", "loc", "k_pool", "v_pool"]),
     ("ce_kv4_read", ["k_pool", "v_pool", "units", "k_out", "v_out"]),
     ("ce_kv4_decode_attn_score", ["q", "k_pool", "v_pool", "kv_indptr", "kv_indices", "kv_tokens", "out", "workspace"]),
-    ("ce_window_decode", ["q", "k_pool", "v_pool", "kv_indptr", "kv_indices", "kv_tokens", "out", "workspace"])])
+    ("ce_window_decode", ["q", "k_pool", "v_pool", "kv_indptr", "kv_indices", "kv_tokens", "out", "workspace"]),
+    ("ce_window_prefill", ["q", "k_pool", "v_pool", "qo_indptr", "kv_indptr", "kv_indices", "kv_tokens", "out"])])
 def test_null_pointers_are_refused(name, pointers):
     for p in pointers:
         assert call(name, null=(p,))[0] == ARG, p
@@ -89,6 +100,8 @@ def test_empty_calls_do_nothing():
     assert call("ce_kv4_read", num_units=0)[0] == OK
     assert call("ce_kv4_decode_attn_score", bs=0)[0] == OK
     assert call("ce_window_decode", bs=0)[0] == OK
+    for none in (dict(bs=0), dict(max_q=0), dict(total_q=0)):
+        assert call("ce_window_prefill", **none)[0] == OK
     assert call("ce_kv4_boundary", num_rows=0)[0] == OK
 
 
@@ -133,6 +146,11 @@ def test_front_end_raises_on_wrong_tensors():
         lambda: kernels.window_decode(q, bf, bf, *csr, 0.125, 16, 8, out=q[:, :32]),
         lambda: kernels.window_decode(q, bf, bf, *csr, 0.125, 16, 8, lse=torch.zeros(3)),
         lambda: kernels.window_decode(q, bf, bf, *csr, 0.125, 16, 8),                  # not on a GPU
+        lambda: kernels.window_prefill(q, bf, bf, csr[0].long(), *csr, 0.125, 16, 1, 1, 8),
+        lambda: kernels.window_prefill(q, bf, bf, csr[0][:1], *csr, 0.125, 16, 1, 1, 8),
+        lambda: kernels.window_prefill(q[0], bf, bf, csr[0], *csr, 0.125, 16, 1, 1, 8),
+        lambda: kernels.window_prefill(q, bf, bf, csr[0], *csr, 0.125, 16, 1, 1, 8, out=q.half()),
+        lambda: kernels.window_prefill(q, bf, bf, csr[0], *csr, 0.125, 16, 1, 1, 8),   # not on a GPU
     ]
     for i, f in enumerate(wrong):
         with pytest.raises(ValueError):
