@@ -1,10 +1,10 @@
 // ce_kv4_decode_attn_score: decode attention and H2O scores over 4-bit pages
 // (the format of ce_kv4.cuh).
 //
-// The batch is split, recorded and combined as for bf16 pages (ce_decode.cu):
-// equal contiguous ranges of stages per CTA, one partial record (m, l, O) per
-// sequence a CTA touched, and the combine kernel over the records.  What is
-// new is the tile.  With k = m_k + c_k s_k and v = m_v + c_v s_v per token,
+// The batch is split as for bf16 pages (ce_decode.cu): equal contiguous ranges
+// of stages per CTA, one partial record (m, l, O) per sequence a CTA touched,
+// merged by a combine kernel.  With k = m_k + c_k s_k and v = m_v + c_v s_v per
+// token,
 //
 //   q . k    = s_k (q . c_k) + m_k sum_d q_d
 //   sum p v  = sum_t (p_t s_t) c_t  +  (sum_t p_t m_t)
@@ -21,6 +21,13 @@
 // are ordinary fp16 numbers.  Rounding them to fp16 (2^-12 relative at most,
 // 2^-39 of the largest) is far below the output's bf16 rounding; logits,
 // maxima, sums and accumulators are fp32.
+//
+// A producer warp copies whole pages (all KV heads) into a ring of shared-memory
+// stages with untiled bulk copies; the format puts a page's fragments in lane
+// order, 16 bytes per lane and operand.  (Loading them from global memory
+// straight into registers a stage ahead needed 221 instructions per page and
+// head instead of 143 and left too few bytes in flight: 178 us instead of 102
+// for 409 MB.)
 #include <algorithm>
 
 #include "ce_decode.cuh"
@@ -31,22 +38,17 @@ namespace kv4 {
 
 using decode::GROUP;
 using decode::LOG2E;
-using decode::NCW;
+using decode::LN2;
 using decode::Params;
-using decode::REC_FLOATS;
-using decode::REC_ROWS;
 
-constexpr int PPW = 4;                               // pages per warp and stage
-constexpr int WT = PPW * P;                          // tokens per warp and stage
-constexpr int HALF_STAGE = NCW * PPW * SLICE;        // 18 KB of K (or V)
-constexpr int STAGE_BYTES = 2 * HALF_STAGE;
-constexpr int NSTAGES = 3;
-constexpr int NPW = 2;                               // producer warps
-constexpr int THREADS = (NCW + NPW) * 32;
-constexpr int SMEM_BYTES = NSTAGES * STAGE_BYTES + 512;
+constexpr int NW = 8;                                // consumer warps
+constexpr int THREADS = (NW + 1) * 32;               // and one producer warp
+constexpr int PPW = 2;                               // pages that a warp computes at a time
 constexpr int CTAS_PER_SM = 2;
-constexpr int MIN_STAGES_LOG2 = 0;
-static_assert(CTAS_PER_SM * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
+constexpr int MIN_STAGES_LOG2 = 0;                   // every CTA below min(stages, grid) has one
+
+// Floats of a record: the unnormalised outputs [H][64], then (maximum, sum) [H].
+__host__ __device__ constexpr int rec_floats(int H) { return H * (D + 2); }
 
 // D += A(16x16) * B(16x8) in fp16 with fp32 accumulation.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -62,14 +64,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
-}
-
-// Untiled bulk copy of `bytes` (a multiple of 16) into shared memory.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_addr(dst)),
-               "l"(src), "r"(bytes), "r"(smem_addr(bar))
-               : "memory");
 }
 
 __device__ __forceinline__ float pow2_bits(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }
@@ -139,8 +133,15 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
   s.kq1 = __shfl_sync(0xffffffffu, kq, 8 * t + 4);
 }
 
+// Untiled bulk copy of `bytes` (a multiple of 16) into shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
+
 struct Side {           // where a scored sequence's page data goes
-  int mode;
   int64_t cpos;         // CSR position of the warp's first page
   int64_t capacity;
   int H, hcol;          // this lane's first head
@@ -149,10 +150,10 @@ struct Side {           // where a scored sequence's page data goes
 
 // PPW pages (the first `ntok` tokens of them) of KV head g: K slices at kb,
 // V slices at vb, one page every `stride` bytes.
-template <bool TAIL>
-__device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* vb, int stride, int ntok, int lane,
+template <int stride, bool TAIL, int MODE>
+__device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* vb, int ntok, int lane,
                                      const Side& side) {
-  const int r = lane >> 2;
+  const int r = lane >> 2, t = lane & 3;
   float u[PPW][4];
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
@@ -173,58 +174,52 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     u[pg][2] = vb2 ? fmaf(sb, c[2], mb * s.qs0) : -INFINITY;
     u[pg][3] = vb2 ? fmaf(sb, c[3], mb * s.qs1) : -INFINITY;
   }
-  float x0 = fmaxf(u[0][0], u[0][2]), x1 = fmaxf(u[0][1], u[0][3]);
-#pragma unroll
-  for (int pg = 1; pg < PPW; ++pg) {
-    x0 = fmaxf(x0, fmaxf(u[pg][0], u[pg][2]));
-    x1 = fmaxf(x1, fmaxf(u[pg][1], u[pg][3]));
-  }
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) {
-    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-  }
-  const float n0 = fmaxf(s.m0, x0 * s.kq0), n1 = fmaxf(s.m1, x1 * s.kq1);
-  const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-  // Rescale the running state only when some head's maximum moved.
-  if (__any_sync(0xffffffffu, n0 != s.m0 || n1 != s.m1)) {
-    const float a0 = fast_exp2(s.m0 - b0), a1 = fast_exp2(s.m1 - b1);
-    s.l0 *= a0;
-    s.l1 *= a1;
-    s.z0 *= a0;
-    s.z1 *= a1;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s.o[q][0] *= a0;
-      s.o[q][1] *= a1;
-      s.o[q][2] *= a0;
-      s.o[q][3] *= a1;
-    }
-    s.m0 = n0;
-    s.m1 = n1;
-  }
-  // V scales and minima; the bound grows (rarely) to stay above every scale.
+  // V scales and minima, and what could move the running state: a logit above
+  // its head's maximum, or a V scale at or above the bound.
   uint2 vp[PPW];
-  float top = 0.f;
+  float x0 = fmaxf(u[0][0], u[0][2]), x1 = fmaxf(u[0][1], u[0][3]), top = 0.f;
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     vp[pg] = *reinterpret_cast<const uint2*>(vb + pg * stride + CODE_BYTES + r * 8);
     if (TAIL && pg * P + 2 * r >= ntok) vp[pg].x = 0u;
     if (TAIL && pg * P + 2 * r + 1 >= ntok) vp[pg].y = 0u;
     top = fmaxf(top, fmaxf(__uint_as_float(vp[pg].x << 16), __uint_as_float(vp[pg].y << 16)));
+    if (pg == 0) continue;
+    x0 = fmaxf(x0, fmaxf(u[pg][0], u[pg][2]));
+    x1 = fmaxf(x1, fmaxf(u[pg][1], u[pg][3]));
   }
-  if (__any_sync(0xffffffffu, top >= s.bound)) {
+  if (__any_sync(0xffffffffu, x0 * s.kq0 > s.m0 || x1 * s.kq1 > s.m1 || top >= s.bound)) {
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float nb = pow2_bits(min(static_cast<int>(__float_as_uint(top) >> 23) + 1, 253));
-    const float f = s.bound * (1.f / nb);
+    for (int o = 4; o < 32; o <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    const float n0 = fmaxf(s.m0, x0 * s.kq0), n1 = fmaxf(s.m1, x1 * s.kq1);
+    const float a0 = n0 == -INFINITY ? 1.f : fast_exp2(s.m0 - n0), a1 = n1 == -INFINITY ? 1.f : fast_exp2(s.m1 - n1);
+    s.m0 = n0;
+    s.m1 = n1;
+    s.l0 *= a0;
+    s.l1 *= a1;
+    s.z0 *= a0;
+    s.z1 *= a1;
+    float f = 1.f;
+    if (top >= s.bound) {   // the same for every lane
+      const float nb = pow2_bits(min(static_cast<int>(__float_as_uint(top) >> 23) + 1, 253));
+      f = s.bound * (1.f / nb);
+      s.bound = nb;
+      s.inv = 32768.f / nb;
+    }
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s.o[q][i] *= f;
-    s.bound = nb;
-    s.inv = 32768.f / nb;
+    for (int q = 0; q < 4; ++q) {
+      s.o[q][0] *= a0 * f;
+      s.o[q][1] *= a1 * f;
+      s.o[q][2] *= a0 * f;
+      s.o[q][3] *= a1 * f;
+    }
   }
+  const float b0 = s.m0 == -INFINITY ? 0.f : s.m0, b1 = s.m1 == -INFINITY ? 0.f : s.m1;
+  float mass[2 * PPW];   // MODE SUM: this lane's share of the pages' masses, heads 2t and 2t + 1
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     float e[4];
@@ -232,32 +227,22 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     e[1] = fast_exp2(fmaf(u[pg][1], s.kq1, -b1));
     e[2] = fast_exp2(fmaf(u[pg][2], s.kq0, -b0));
     e[3] = fast_exp2(fmaf(u[pg][3], s.kq1, -b1));
-    const float t0 = e[0] + e[2], t1 = e[1] + e[3];
-    s.l0 += t0;
-    s.l1 += t1;
+    mass[2 * pg] = e[0] + e[2];
+    mass[2 * pg + 1] = e[1] + e[3];
+    s.l0 += mass[2 * pg];
+    s.l1 += mass[2 * pg + 1];
     const float sa = __uint_as_float(vp[pg].x << 16) * s.inv, ma = __uint_as_float(vp[pg].x & 0xffff0000u);
     const float sb = __uint_as_float(vp[pg].y << 16) * s.inv, mb = __uint_as_float(vp[pg].y & 0xffff0000u);
     s.z0 = fmaf(e[0], ma, fmaf(e[2], mb, s.z0));
     s.z1 = fmaf(e[1], ma, fmaf(e[3], mb, s.z1));
     const uint32_t p0 = movmatrix_trans(pack_f16(e[0] * sa, e[1] * sa));
     const uint32_t p1 = movmatrix_trans(pack_f16(e[2] * sb, e[3] * sb));
-    const uint4 w = *reinterpret_cast<const uint4*>(vb + pg * stride + ((lane & 3) * 8 + r) * 16);
+    const uint4 w = *reinterpret_cast<const uint4*>(vb + pg * stride + (t * 8 + r) * 16);
     const uint32_t wq[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       mma_f16(s.o[q], wq[q] & LOW, wq[q] & HIGH, (wq[q] >> 8) & LOW, (wq[q] >> 8) & HIGH, p0, p1);
-    if (side.mode == CE_MODE_SUM) {
-      // log2 of the page's mass under the running maximum
-      float y0 = t0, y1 = t1;
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        y0 += __shfl_xor_sync(0xffffffffu, y0, o);
-        y1 += __shfl_xor_sync(0xffffffffu, y1, o);
-      }
-      if (r == 0 && (!TAIL || pg * P < ntok) && side.cpos + pg < side.capacity)
-        *reinterpret_cast<float2*>(side.ul + (side.cpos + pg) * side.H + side.hcol) =
-            make_float2(y0 > 0.f ? b0 + __log2f(y0) : -INFINITY, y1 > 0.f ? b1 + __log2f(y1) : -INFINITY);
-    } else if (side.mode == CE_MODE_MAX) {
+    if (MODE == CE_MODE_MAX) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int j = 2 * r + h;
@@ -267,11 +252,29 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
       }
     }
   }
+  if (MODE == CE_MODE_SUM) {
+    // Sum the 4 (page, head) shares over the lanes of equal t; each step halves
+    // what a lane still carries, and lanes (r, t) of equal r / 2 end with page
+    // r / 4, head 2t + r / 2 % 2, whose log2 mass under the running maximum they keep.
+    static_assert(PPW == 2, "four shares over eight lanes");
+    float h2[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float mine = (r & 4) ? mass[2 + i] : mass[i], yours = (r & 4) ? mass[i] : mass[2 + i];
+      h2[i] = mine + __shfl_xor_sync(0xffffffffu, yours, 16);
+    }
+    const float mine = (r & 2) ? h2[1] : h2[0], yours = (r & 2) ? h2[0] : h2[1];
+    float y = mine + __shfl_xor_sync(0xffffffffu, yours, 8);
+    y += __shfl_xor_sync(0xffffffffu, y, 4);
+    const int pg = r >> 2, h = (r >> 1) & 1;
+    if (!(r & 1) && (!TAIL || pg * P < ntok) && side.cpos + pg < side.capacity)
+      side.ul[(side.cpos + pg) * side.H + side.hcol + h] = y > 0.f ? (h ? b1 : b0) + __log2f(y) : -INFINITY;
+  }
 }
 
-// The warp's record of a sequence, in the layout of ce_decode.cu's records.
-__device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp, int lane) {
-  const int r = lane >> 2, t = lane & 3;
+// The warp's sums over its lanes, and its output row in place: head 2t of dims
+// 16 q + r (i = 0) and 16 q + r + 8 (i = 2), head 2t + 1 likewise (i = 1, 3).
+__device__ __forceinline__ void finish(Rows& s) {
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
     s.l0 += __shfl_xor_sync(0xffffffffu, s.l0, o);
@@ -279,53 +282,157 @@ __device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp,
     s.z0 += __shfl_xor_sync(0xffffffffu, s.z0, o);
     s.z1 += __shfl_xor_sync(0xffffffffu, s.z1, o);
   }
-  float* rec = p.rec + static_cast<int64_t>(b + blockIdx.x) * REC_FLOATS;
-  const int v0 = warp * 8 + 2 * t;
   // accumulators hold sum (p s 2^15 / bound) (c 2^-24), upper nibbles 16-fold;
   // bound 2^9 in two steps that cannot overflow
   const float fb = s.bound * 9.5367431640625e-7f;   // 2^-20
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    rec[v0 * D + q * 16 + r] = fmaf(s.o[q][0] * 536870912.f, fb, s.z0);
-    rec[(v0 + 1) * D + q * 16 + r] = fmaf(s.o[q][1] * 536870912.f, fb, s.z1);
-    rec[v0 * D + q * 16 + r + 8] = fmaf(s.o[q][2] * 33554432.f, fb, s.z0);
-    rec[(v0 + 1) * D + q * 16 + r + 8] = fmaf(s.o[q][3] * 33554432.f, fb, s.z1);
-  }
-  if (r == 0) {
-    rec[REC_ROWS * D + v0] = s.m0;
-    rec[REC_ROWS * D + v0 + 1] = s.m1;
-    rec[REC_ROWS * D + REC_ROWS + v0] = s.l0;
-    rec[REC_ROWS * D + REC_ROWS + v0 + 1] = s.l1;
+    s.o[q][0] = fmaf(s.o[q][0] * 536870912.f, fb, s.z0);
+    s.o[q][1] = fmaf(s.o[q][1] * 536870912.f, fb, s.z1);
+    s.o[q][2] = fmaf(s.o[q][2] * 33554432.f, fb, s.z0);
+    s.o[q][3] = fmaf(s.o[q][3] * 33554432.f, fb, s.z1);
   }
 }
+
+// A warp's heads into rows h0 .. h0 + 7 of a record-shaped buffer of H heads.
+__device__ __forceinline__ void put(const Rows& s, float* rec, int H, int h0, int lane) {
+  const int r = lane >> 2, t = lane & 3;
+  float* o = rec + (h0 + 2 * t) * D + r;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    o[q * 16] = s.o[q][0];
+    o[D + q * 16] = s.o[q][1];
+    o[q * 16 + 8] = s.o[q][2];
+    o[D + q * 16 + 8] = s.o[q][3];
+  }
+  if (r == 0) {
+    float* ml = rec + H * D + (h0 + 2 * t) * 2;
+    ml[0] = s.m0;
+    ml[1] = s.l0;
+    ml[2] = s.m1;
+    ml[3] = s.l1;
+  }
+}
+
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory"); }
+
+// The CTA's record of a sequence.  Below 8 KV heads several warps share a head:
+// their parts are merged in shared memory, so that a record has one row per
+// head whatever the split.
+template <int G>
+__device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp, int lane, float* part) {
+  constexpr int H = G * GROUP, SUB = NW / G;
+  float* rec = p.rec + static_cast<int64_t>(b + blockIdx.x) * rec_floats(H);
+  finish(s);
+  if constexpr (SUB == 1) {
+    put(s, rec, H, warp * GROUP, lane);
+    return;
+  }
+  consumers_sync();   // the buffer is free (all warps leave the same sequences in the same order)
+  put(s, part + (warp / G) * rec_floats(H), H, (warp % G) * GROUP, lane);
+  consumers_sync();
+  for (int i = threadIdx.x; i < H * D / 2; i += NW * 32) {
+    const int h = i / (D / 2);
+    float m[SUB], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < SUB; ++k) {
+      m[k] = part[k * rec_floats(H) + H * D + 2 * h];
+      top = fmaxf(top, m[k]);
+    }
+    float2 o = make_float2(0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int k = 0; k < SUB; ++k) {
+      const float* q = part + k * rec_floats(H);
+      const float w = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - top);
+      const float2 x = reinterpret_cast<const float2*>(q)[i];
+      o.x += w * x.x;
+      o.y += w * x.y;
+      l += w * q[H * D + 2 * h + 1];
+    }
+    reinterpret_cast<float2*>(rec)[i] = o;
+    if (i % (D / 2) == 0) {
+      rec[H * D + 2 * h] = top;
+      rec[H * D + 2 * h + 1] = l;
+    }
+  }
+}
+
+// The batch's stages in order: sequence b from stage `base` on, its tokens and
+// first CSR position; the next sequence's are loaded one sequence ahead.
+template <int ST>
+struct Cursor {
+  int b, base, tok, nst, next_tok;
+  int64_t ip, next_ip;
+  __device__ __forceinline__ void fetch_next(const Params& p) {
+    const bool more = b + 1 < p.bs;
+    next_tok = more ? decode::seq_tokens(p, b + 1, P) : 0;
+    next_ip = more ? p.kv_indptr[b + 1] : 0;
+  }
+  __device__ __forceinline__ void start(const Params& p, int bb, int first) {
+    b = bb;
+    base = first;
+    tok = b < p.bs ? decode::seq_tokens(p, b, P) : 0;
+    ip = b < p.bs ? p.kv_indptr[b] : 0;
+    nst = (tok + ST - 1) / ST;
+    fetch_next(p);
+  }
+  __device__ __forceinline__ void to(const Params& p, int x) {   // x below the batch's stages
+    while (x >= base + nst) {
+      base += nst;
+      ++b;
+      tok = next_tok;
+      ip = next_ip;
+      nst = (tok + ST - 1) / ST;
+      fetch_next(p);
+    }
+  }
+};
+
+// Sizes that go with G KV heads: a stage is WT tokens of every consumer warp.
+// Below 8 heads several warps share a head and leave() needs a buffer, so
+// stages are halved there to keep two CTAs on an SM.
+template <int G>
+struct Shape {
+  static constexpr int H = G * GROUP, SUB = NW / G;
+  static constexpr int WT = (SUB == 1 ? 4 : 2) * P;
+  static constexpr int ST = WT * SUB, UPS = ST / P;
+  static constexpr int UNIT_BYTES = G * SLICE;
+  static constexpr int HALF_STAGE = UPS * UNIT_BYTES, STAGE_BYTES = 2 * HALF_STAGE;   // K, then V
+  static constexpr int NSTAGES = SUB == 1 ? 3 : 5;
+  static constexpr int SMEM = NSTAGES * STAGE_BYTES + (SUB == 1 ? 0 : SUB * rec_floats(H) * 4);
+  static_assert(CTAS_PER_SM * (SMEM + 2048) <= 228 * 1024, "two CTAs per SM");
+};
 
 __device__ __forceinline__ int stages_of(const Params& p, int b, int ST) {
   return (decode::seq_tokens(p, b, P) + ST - 1) / ST;
 }
 
-// Warps 0..7 consume (warp w: KV head w % G, pages 4 (w / G) .. +3 of each
-// stage), warps 8.. produce (stage k by warp 8 + k % NPW).
+// Warps 0..7 consume (warp w: KV head w % G, every (8 / G)-th group of pages
+// of each stage), warp 8 produces.
+template <int G>
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     attn_kernel(const Params p, const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool) {
+  using C = Shape<G>;
+  constexpr int H = C::H, WT = C::WT, ST = C::ST, UPS = C::UPS, UNIT_BYTES = C::UNIT_BYTES;
+  constexpr int NSTAGES = C::NSTAGES, STAGE_BYTES = C::STAGE_BYTES, HALF_STAGE = C::HALF_STAGE;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + NSTAGES * STAGE_BYTES);
-  uint64_t* empty = full + NSTAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + NSTAGES);
-  int* start_sh = reinterpret_cast<int*>(smem + NSTAGES * STAGE_BYTES + 64);
-  int64_t* scan_sh = reinterpret_cast<int64_t*>(smem + NSTAGES * STAGE_BYTES + 128);
+  float* part = reinterpret_cast<float*>(smem + NSTAGES * STAGE_BYTES);   // leave()
+  __shared__ uint64_t full[NSTAGES], empty[NSTAGES];
+  __shared__ int64_t scan_sh[32];
+  __shared__ int start_sh[2], abort_sh;
+  volatile int* abort_flag = &abort_sh;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = p.G, H = p.H;
-  const int ST = WT * (NCW / G);            // tokens per stage
-  const int UPS = ST / P;                   // pages per stage
-  const int unit_bytes = G * SLICE;
 
   if (tid == 0) {
     for (int s = 0; s < NSTAGES; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], NCW);
+      mbar_init(&empty[s], NW);
     }
     *abort_flag = 0;
+    start_sh[0] = p.bs;
+    start_sh[1] = 0;
     fence_mbar_init();
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -337,24 +444,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   int64_t local = 0;
   for (int b = lo_b; b < hi_b; ++b) local += stages_of(p, b, ST);
   int64_t S = 0;
-  const int64_t excl = decode::block_excl_scan(local, scan_sh, S);
+  const int64_t excl = decode::block_excl_scan(local, scan_sh, S);   // a barrier: start_sh is set
   const int64_t k = blockIdx.x, grid = decode::eff_grid(S, gridDim.x, MIN_STAGES_LOG2);
   const int64_t S_lo = k < grid ? k * S / grid : S, S_hi = k < grid ? (k + 1) * S / grid : S;
-  if (blockIdx.x == 0) {
-    int64_t run = excl;
-    for (int b = lo_b; b < hi_b; ++b) {
-      p.prefix[b] = static_cast<int32_t>(run);
-      const int n = stages_of(p, b, ST);
-      run += n;
-      if (n == 0) decode::empty_sequence(p, b);
-    }
-    if (tid == 0) p.prefix[bs] = static_cast<int32_t>(S);
-  }
-  if (tid == 0) {
-    start_sh[0] = bs;
-    start_sh[1] = 0;
-  }
-  __syncthreads();
   if (S_lo < S_hi && excl <= S_lo && S_lo < excl + local) {
     int64_t run = excl;
     for (int b = lo_b; b < hi_b; ++b) {
@@ -368,6 +460,15 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     }
   }
   __syncthreads();
+  if (blockIdx.x == 0) {
+    int64_t run = excl;
+    for (int b = lo_b; b < hi_b; ++b) {
+      p.prefix[b] = static_cast<int32_t>(run);
+      const int n = stages_of(p, b, ST);
+      run += n;
+    }
+    if (tid == 0) p.prefix[bs] = static_cast<int32_t>(S);
+  }
 
   int b = start_sh[0], base = start_sh[1];
   int nst = 0, tok_b = 0;
@@ -379,10 +480,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   };
   if (b < bs) load_seq(b);
 
-  if (warp >= NCW) {
-    // ------------------------------- producers -------------------------------
+  if (warp == NW) {
+    // -------------------------------- producer --------------------------------
     // Page indices in 32-entry windows, a third one in flight, as for bf16 pages.
-    const int pw = warp - NCW;
     int issued = 0;
     auto fetch = [&](int64_t w0) -> int {
       const int64_t c = w0 + lane;
@@ -390,13 +490,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     };
     int64_t w0 = -1;
     int idx_cur = -2, idx_next = -2, idx_ahead = -2;
-    for (int64_t x = S_lo; x < S_hi; ++x) {
+    for (int64_t x = S_lo; x < S_hi; ++x, ++issued) {
       while (x >= base + nst) {
         base += nst;
         ++b;
         load_seq(b);
       }
-      if (*abort_flag) break;
       const int j = static_cast<int>(x - base);
       const int ntok = min(ST, tok_b - j * ST);
       const int nunits = (ntok + P - 1) / P;
@@ -413,18 +512,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
         idx_ahead = fetch(w0 + 64);
       }
       const int s = issued % NSTAGES;
-      if (issued % NPW != pw) {
-        ++issued;
-        continue;
-      }
-      if (issued >= NSTAGES) {
-        bool ok = true;
-        if (lane == 0) ok = mbar_wait_or_abort(&empty[s], ((issued / NSTAGES) & 1) ^ 1, p.err, abort_flag);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) {
-          *abort_flag = 1;
-          break;
-        }
+      if (issued >= NSTAGES && !warp_wait(&empty[s], ((issued / NSTAGES) & 1) ^ 1, p.err, abort_flag, lane)) {
+        *abort_flag = 1;
+        break;
       }
       const int slot = static_cast<int>(c0 - w0) + lane;
       const int a = __shfl_sync(0xffffffffu, idx_cur, slot & 31);
@@ -441,28 +531,25 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
         }
       }
       const unsigned valid = __ballot_sync(0xffffffffu, unit >= 0);
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(valid) * unit_bytes * 2);
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(valid) * UNIT_BYTES * 2);
       __syncwarp();
       if (unit >= 0) {
-        uint8_t* kd = smem + s * STAGE_BYTES + lane * unit_bytes;
-        const int64_t off = static_cast<int64_t>(unit) * unit_bytes;
-        bulk_load(kd, k_pool + off, unit_bytes, &full[s]);
-        bulk_load(kd + HALF_STAGE, v_pool + off, unit_bytes, &full[s]);
+        uint8_t* kd = smem + s * STAGE_BYTES + lane * UNIT_BYTES;
+        const int64_t off = static_cast<int64_t>(unit) * UNIT_BYTES;
+        bulk_load(kd, k_pool + off, UNIT_BYTES, &full[s]);
+        bulk_load(kd + HALF_STAGE, v_pool + off, UNIT_BYTES, &full[s]);
       }
-      ++issued;
     }
-    // Every load this warp issued lands before the CTA may exit.
-    if (lane == 0) {
-      for (int it = max(0, issued - NSTAGES); it < issued; ++it)
-        if (it % NPW == pw) mbar_wait(&full[it % NSTAGES], (it / NSTAGES) & 1, p.err);
-    }
+    // Every load issued lands before the CTA may exit.
+    if (lane == 0)
+      for (int it = max(0, issued - NSTAGES); it < issued; ++it) mbar_wait(&full[it % NSTAGES], (it / NSTAGES) & 1, p.err);
   } else {
     // ------------------------------- consumers -------------------------------
     const int g = warp % G, tb = warp / G;
     const int head = g * GROUP + (lane >> 2);
     Rows st;
-    Side side{CE_MODE_NONE, 0, p.kv_capacity, H, g * GROUP + 2 * (lane & 3), p.ul, p.tl};
-    int cur_b = -1, s = 0;
+    Side side{0, p.kv_capacity, H, g * GROUP + 2 * (lane & 3), p.ul, p.tl};
+    int cur_b = -1, mode = CE_MODE_NONE, s = 0;
     uint32_t ph = 0;
     bool aborted = false;
     for (int64_t x = S_lo; x < S_hi; ++x) {
@@ -472,16 +559,15 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
         load_seq(b);
       }
       if (b != cur_b) {
-        if (cur_b >= 0) leave(p, st, cur_b, warp, lane);
+        if (cur_b >= 0) leave<G>(p, st, cur_b, warp, lane, part);
         cur_b = b;
         clear(st);
         load_query(st, p.q + static_cast<int64_t>(b) * p.q_sb + static_cast<int64_t>(head) * p.q_sh, lane & 3,
                    p.scale_log2);
-        side.mode = decode::seq_mode(p, b);
-        if (side.mode != CE_MODE_SUM && side.mode != CE_MODE_MAX) side.mode = CE_MODE_NONE;
-        if ((side.mode == CE_MODE_SUM && !p.ul) || (side.mode == CE_MODE_MAX && !p.tl)) {
+        mode = decode::seq_mode(p, b);
+        if ((mode == CE_MODE_SUM && !p.ul) || (mode == CE_MODE_MAX && !p.tl)) {
           if (lane == 0 && warp == 0) flag_error(p.err, CE_EW_MODE);
-          side.mode = CE_MODE_NONE;
+          mode = CE_MODE_NONE;
         }
       }
       const int j = static_cast<int>(x - base);
@@ -499,18 +585,239 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
         aborted = true;
       }
       if (aborted) continue;
-      const uint8_t* kb = smem + cs * STAGE_BYTES + tb * PPW * unit_bytes + g * SLICE;
-      side.cpos = ip_b + static_cast<int64_t>(j) * UPS + tb * PPW;
-      if (mine >= WT)
-        tile<false>(st, kb, kb + HALF_STAGE, unit_bytes, WT, lane, side);
-      else if (mine > 0)
-        tile<true>(st, kb, kb + HALF_STAGE, unit_bytes, mine, lane, side);
+      const uint8_t* kb = smem + cs * STAGE_BYTES + tb * (WT / P) * UNIT_BYTES + g * SLICE;
+      const uint8_t* vb = kb + HALF_STAGE;
+      side.cpos = ip_b + static_cast<int64_t>(j) * UPS + tb * (WT / P);
+      constexpr int STEP = PPW * P;
+#pragma unroll 1
+      for (int left = mine; left > max(mine - WT, 0); left -= STEP) {
+        if (left >= STEP) {
+          if (mode == CE_MODE_SUM) tile<UNIT_BYTES, false, CE_MODE_SUM>(st, kb, vb, STEP, lane, side);
+          else if (mode == CE_MODE_MAX) tile<UNIT_BYTES, false, CE_MODE_MAX>(st, kb, vb, STEP, lane, side);
+          else tile<UNIT_BYTES, false, CE_MODE_NONE>(st, kb, vb, STEP, lane, side);
+        } else {
+          if (mode == CE_MODE_SUM) tile<UNIT_BYTES, true, CE_MODE_SUM>(st, kb, vb, left, lane, side);
+          else if (mode == CE_MODE_MAX) tile<UNIT_BYTES, true, CE_MODE_MAX>(st, kb, vb, left, lane, side);
+          else tile<UNIT_BYTES, true, CE_MODE_NONE>(st, kb, vb, left, lane, side);
+        }
+        kb += PPW * UNIT_BYTES;
+        vb += PPW * UNIT_BYTES;
+        side.cpos += PPW;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[cs]);   // release orders the reads above
     }
-    if (cur_b >= 0) leave(p, st, cur_b, warp, lane);
+    if (cur_b >= 0) leave<G>(p, st, cur_b, warp, lane, part);
   }
   __syncthreads();
+}
+
+// Output, normaliser and log2 normaliser of every (row, head) from its records:
+// W warps each merge every W-th group of slots (lane i: slot i's maximum and
+// sum; then the slots' output rows, two dims per lane).
+constexpr int CB_THREADS = 256;
+
+template <int H, int W>
+__global__ void __launch_bounds__(CB_THREADS) combine_kernel(const Params p, int launched) {
+  constexpr int PER = CB_THREADS / 32 / W;   // (row, head) pairs per block
+  __shared__ float sh_o[W > 1 ? W : 1][D], sh_ml[W > 1 ? W : 1][2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % W;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * PER + warp / W;
+  if (item >= static_cast<int64_t>(p.bs) * H) return;   // the whole block when W > 1
+  const int b = static_cast<int>(item / H), h = static_cast<int>(item % H);
+  const int64_t S = p.prefix[p.bs], pre = p.prefix[b], n = p.prefix[b + 1] - pre;
+  const int64_t grid = decode::eff_grid(S, launched, MIN_STAGES_LOG2);
+  int k0 = 0, slots = 0;
+  if (n > 0) {
+    k0 = decode::cta_of_stage(pre, S, grid);
+    slots = decode::cta_of_stage(pre + n - 1, S, grid) - k0 + 1;
+  }
+  const float* rec = p.rec + static_cast<int64_t>(b + k0) * rec_floats(H);
+  float m = -INFINITY, l = 0.f;
+  float2 o = make_float2(0.f, 0.f);
+  constexpr int BATCH = W > 1 ? 8 : 32;   // slots per round
+  for (int s0 = sub * BATCH; s0 < slots; s0 += W * BATCH) {
+    const int cnt = min(BATCH, slots - s0);
+    const float* base = rec + static_cast<int64_t>(s0) * rec_floats(H);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < cnt) ml = *reinterpret_cast<const float2*>(base + static_cast<int64_t>(lane) * rec_floats(H) + H * D + 2 * h);
+    float top = ml.x;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    top = fmaxf(top, m);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+    float sum = w * ml.y;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const float a = m == -INFINITY ? 0.f : exp2f(m - top);
+    l = l * a + sum;
+    o.x *= a;
+    o.y *= a;
+    m = top;
+    for (int i0 = 0; i0 < cnt; i0 += 8) {
+      float2 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = make_float2(0.f, 0.f);
+        if (i0 + i < cnt)
+          v[i] = *reinterpret_cast<const float2*>(base + static_cast<int64_t>(i0 + i) * rec_floats(H) + h * D + 2 * lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
+        if (i0 + i < cnt) {
+          o.x = fmaf(wi, v[i].x, o.x);
+          o.y = fmaf(wi, v[i].y, o.y);
+        }
+      }
+    }
+  }
+  if constexpr (W > 1) {
+    reinterpret_cast<float2*>(sh_o[warp])[lane] = o;
+    if (lane == 0) {
+      sh_ml[warp][0] = m;
+      sh_ml[warp][1] = l;
+    }
+    __syncthreads();
+    if (warp > 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < W; ++k) m = fmaxf(m, sh_ml[k][0]);
+    l = 0.f;
+    o = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float a = sh_ml[k][0] == -INFINITY ? 0.f : exp2f(sh_ml[k][0] - m);
+      const float2 x = reinterpret_cast<const float2*>(sh_o[k])[lane];
+      l += a * sh_ml[k][1];
+      o.x = fmaf(a, x.x, o.x);
+      o.y = fmaf(a, x.y, o.y);
+    }
+  }
+  // with the sink in the normaliser; a row with neither tokens nor a sink is
+  // zeros and -inf
+  const float sink2 = p.sinks ? p.sinks[h] * LOG2E : -INFINITY;
+  const float top = fmaxf(m, sink2);
+  float L = -INFINITY, f = 0.f;
+  if (n > 0 || sink2 != -INFINITY) {
+    const float a = m == -INFINITY ? (l != l ? l : 0.f) : exp2f(m - top);   // a row of NaN logits has no maximum
+    const float den = l * a + (p.sinks ? exp2f(sink2 - top) : 0.f);
+    L = top + log2f(den);
+    f = a / den;
+  }
+  const int64_t at = static_cast<int64_t>(b) * p.o_sb + static_cast<int64_t>(h) * p.o_sh + 2 * lane;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + at;
+  out[0] = __float2bfloat16_rn(n > 0 ? o.x * f : 0.f);
+  out[1] = __float2bfloat16_rn(n > 0 ? o.y * f : 0.f);
+  if (lane == 0) {
+    p.lse2[item] = L;
+    if (p.lse_out) p.lse_out[item] = L * LN2;
+  }
+}
+
+// Page scores of the batch from the combine kernel's normalisers: scores[g, unit]
+// += SUM: sum_h 2^(page log-mass - L_h), MAX: sum_t 2^(max_h (s_t,h - L_h)).  Block
+// (x, b) takes every gridDim.x-th group of pages of row b, all KV heads at
+// once, so that neighbouring threads read neighbouring heads and pages.
+constexpr int SC_THREADS = 256;
+
+template <int G>
+__global__ void __launch_bounds__(SC_THREADS) score_kernel(const Params p) {
+  constexpr int H = G * GROUP;
+  const int b = blockIdx.y;
+  const int mode = decode::seq_mode(p, b);
+  if ((mode != CE_MODE_SUM || !p.ul) && (mode != CE_MODE_MAX || !p.tl)) return;
+  const int tokens = decode::seq_tokens(p, b, P);
+  const int npages = (tokens + P - 1) / P;
+  const int64_t ip = p.kv_indptr[b];
+  const int fresh = p.zero_new && (tokens - 1) % P == 0 ? npages - 1 : -1;
+  const int lane = threadIdx.x & 31;
+  const int g = lane % G;
+  float L[GROUP];
+  {
+    const float4* l4 = reinterpret_cast<const float4*>(p.lse2 + static_cast<int64_t>(b) * H + g * GROUP);
+    const float4 x = l4[0], y = l4[1];
+    L[0] = x.x, L[1] = x.y, L[2] = x.z, L[3] = x.w, L[4] = y.x, L[5] = y.y, L[6] = y.z, L[7] = y.w;
+  }
+  float* sc = p.scores + g * p.score_sg;
+  auto add = [&](int j, float mass) {
+    const int unit = p.kv_indices[ip + j];
+    if (unit < 0 || unit >= p.pool_units) return;   // flagged by the attention kernel
+    sc[unit] = j == fresh ? mass : sc[unit] + mass;
+  };
+  if (mode == CE_MODE_SUM) {
+    constexpr int PB = SC_THREADS / G;   // pages per block and round
+    for (int j = blockIdx.x * PB + threadIdx.x / G; j < npages; j += gridDim.x * PB) {
+      if (ip + j >= p.kv_capacity) break;
+      const float4* u4 = reinterpret_cast<const float4*>(p.ul + (ip + j) * H + g * GROUP);
+      const float4 x = u4[0], y = u4[1];
+      const float u[GROUP] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      float mass = 0.f;
+#pragma unroll
+      for (int r = 0; r < GROUP; ++r) mass += fast_exp2(u[r] - L[r]);
+      add(j, mass);
+    }
+    return;
+  }
+  // A warp's lanes are token lanes x heads: a page takes TL of them (one page
+  // per warp, two at G = 1), TPL tokens each.
+  constexpr int LANES = 32 / G, TL = LANES < P ? LANES : P, TPL = P / TL, PW = LANES / TL;
+  const int tl = (lane / G) % TL, pw = lane / (G * TL);
+  const int step = gridDim.x * (SC_THREADS / 32) * PW;
+  for (int j0 = (blockIdx.x * (SC_THREADS / 32) + (threadIdx.x >> 5)) * PW; j0 < npages; j0 += step) {
+    const int j = j0 + pw;
+    const bool in = j < npages && ip + j < p.kv_capacity;
+    float mass = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) {
+      const int t = tl + i * TL;
+      if (in && j * P + t < tokens) {
+        const float4* u4 = reinterpret_cast<const float4*>(p.tl + ((ip + j) * P + t) * H + g * GROUP);
+        const float4 x = u4[0], y = u4[1];
+        const float top = fmaxf(fmaxf(fmaxf(x.x - L[0], x.y - L[1]), fmaxf(x.z - L[2], x.w - L[3])),
+                                fmaxf(fmaxf(y.x - L[4], y.y - L[5]), fmaxf(y.z - L[6], y.w - L[7])));
+        mass += fast_exp2(top);
+      }
+    }
+#pragma unroll
+    for (int o = G; o < G * TL; o <<= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    if (in && tl == 0) add(j, mass);
+  }
+}
+
+template <int G>
+int launch(const Params& p, const uint8_t* k_pool, const uint8_t* v_pool, int sms, int score_flags, cudaStream_t st) {
+  constexpr int H = G * GROUP;
+  const int grid = CTAS_PER_SM * sms;
+  if (!host::set_smem(attn_kernel<G>, Shape<G>::SMEM)) return host::fail(CE_ERR_CUDA, "smem attr");
+  attn_kernel<G><<<grid, THREADS, Shape<G>::SMEM, st>>>(p, k_pool, v_pool);
+  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_kv4_decode launch");
+  // Few (row, head) pairs have many records each (a row spans many CTAs): a
+  // block per pair; many pairs a warp each.
+  const int64_t pairs = static_cast<int64_t>(p.bs) * H;
+  if (pairs <= 8LL * sms)
+    combine_kernel<H, 8><<<static_cast<unsigned>(pairs), CB_THREADS, 0, st>>>(p, grid);
+  else
+    combine_kernel<H, 1><<<static_cast<unsigned>((pairs + 7) / 8), CB_THREADS, 0, st>>>(p, grid);
+  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_kv4_decode combine launch");
+  if ((score_flags & CE_SCORE_DEFER) || !(score_flags & 3) || !p.mode_of_row) return CE_OK;
+  // The scores are a launch of their own over all pages, about four blocks per
+  // SM over the batch (a task per row and head, as inside the bf16 combine,
+  // left the longest row's pages to one block: 371 us instead of 214).
+  const int x = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((4LL * sms + p.bs - 1) / p.bs, 512)));
+  score_kernel<G><<<dim3(x, p.bs), SC_THREADS, 0, st>>>(p);
+  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_kv4_decode score launch");
+  return CE_OK;
+}
+
+template <int G>
+int load() {
+  cudaFuncAttributes a;
+  return host::set_smem(attn_kernel<G>, Shape<G>::SMEM) &&
+                 cudaFuncGetAttributes(&a, combine_kernel<G * GROUP, 1>) == cudaSuccess &&
+                 cudaFuncGetAttributes(&a, combine_kernel<G * GROUP, 8>) == cudaSuccess &&
+                 cudaFuncGetAttributes(&a, score_kernel<G>) == cudaSuccess
+             ? CE_OK : CE_ERR_CUDA;
 }
 
 }  // namespace kv4
@@ -522,7 +829,7 @@ namespace {
 int check_shape(int32_t bs, int64_t pool_units, int64_t cap, int32_t H, int32_t G, int32_t head_dim, int32_t page_size) {
   if (bs < 0 || pool_units < 0 || cap < 0) return host::fail(CE_ERR_ARG, "ce_kv4_decode: negative size");
   if (head_dim != kv4::D) return host::fail(CE_ERR_UNSUPPORTED, "ce_kv4_decode: head_dim must be 64");
-  if (G <= 0 || H != kv4::GROUP * G || kv4::NCW % G != 0)
+  if (G <= 0 || H != kv4::GROUP * G || kv4::NW % G != 0)
     return host::fail(CE_ERR_UNSUPPORTED, "ce_kv4_decode: needs 8 query heads per KV head and 1/2/4/8 KV heads");
   if (page_size != kv4::P) return host::fail(CE_ERR_UNSUPPORTED, "ce_kv4_decode: page_size must be 16");
   return CE_OK;
@@ -551,6 +858,7 @@ extern "C" int ce_kv4_decode_attn_score(const void* q, int64_t q_sb, int64_t q_s
   if (shape != CE_OK) return shape;
   if (!(sm_scale > 0.f)) return host::fail(CE_ERR_ARG, "ce_kv4_decode: sm_scale must be positive");
   if (bs == 0) return CE_OK;
+  if (bs > 65535) return host::fail(CE_ERR_UNSUPPORTED, "ce_kv4_decode: more than 65535 rows");
   if (!q || !k_pool || !v_pool || !kv_indptr || !kv_indices || !kv_tokens || !out || !workspace)
     return host::fail(CE_ERR_ARG, "ce_kv4_decode: null pointer");
   if (pool_units == 0) return host::fail(CE_ERR_ARG, "ce_kv4_decode: empty pool");
@@ -600,14 +908,17 @@ extern "C" int ce_kv4_decode_attn_score(const void* q, int64_t q_sb, int64_t q_s
   p.window = -1;
   p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!host::set_smem(kv4::attn_kernel, kv4::SMEM_BYTES)) return host::fail(CE_ERR_CUDA, "smem attr");
-  kv4::attn_kernel<<<grid, kv4::THREADS, kv4::SMEM_BYTES, st>>>(p, static_cast<const uint8_t*>(k_pool),
-                                                                static_cast<const uint8_t*>(v_pool));
-  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_kv4_decode launch");
-  return host::launch_combine(p, grid, kv4::P, (score_flags & CE_SCORE_DEFER) != 0, st);
+  const uint8_t *kp = static_cast<const uint8_t*>(k_pool), *vp = static_cast<const uint8_t*>(v_pool);
+  switch (num_kv_heads) {
+    case 1: return kv4::launch<1>(p, kp, vp, sms, score_flags, st);
+    case 2: return kv4::launch<2>(p, kp, vp, sms, score_flags, st);
+    case 4: return kv4::launch<4>(p, kp, vp, sms, score_flags, st);
+    default: return kv4::launch<8>(p, kp, vp, sms, score_flags, st);
+  }
 }
 
 int ce::host::kv4_prepare_device() {
-  if (!host::set_smem(kv4::attn_kernel, kv4::SMEM_BYTES)) return host::fail_cuda("4-bit decode kernel: set-up");
+  if (kv4::load<1>() != CE_OK || kv4::load<2>() != CE_OK || kv4::load<4>() != CE_OK || kv4::load<8>() != CE_OK)
+    return host::fail_cuda("4-bit decode kernels: set-up");
   return host::kv4_copy_prepare_device();
 }
