@@ -17,8 +17,8 @@
 // two K-steps' halves of K, for four ANDs and a shift.  The other operand
 // brings the range back: the query row is scaled by a power of two to
 // 2^14 .. 2^15 (1/16 of that where it meets upper nibbles), and the weights
-// p_t s_t by 2^15 over a power of two above every scale seen so far, so both
-// are ordinary fp16 numbers.  Rounding them to fp16 (2^-12 relative at most,
+// p_t s_t by 2^15 over a power of two above every scale seen so far (in the
+// exponent of p_t itself), so both are ordinary fp16 numbers.  Rounding them to fp16 (2^-12 relative at most,
 // 2^-39 of the largest) is far below the output's bf16 rounding; logits,
 // maxima, sums and accumulators are fp32.
 //
@@ -53,10 +53,18 @@ __host__ __device__ constexpr int rec_floats(int H) { return H * (D + 2); }
 // D += A(16x16) * B(16x8) in fp16 with fp32 accumulation.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with D = A * B.
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // (lo, hi) as fp16x2, lo in the low half.
@@ -64,6 +72,31 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Pairs of fp32 in one 64-bit register, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void split(uint64_t d, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 __device__ __forceinline__ float pow2_bits(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }
@@ -76,21 +109,26 @@ struct Rows {
   uint32_t qb[4][2];    // B operand of S^T: query codes' partners, fp16
   float qs0, qs1;       // 2^-24 sum of the scaled query row
   float kq0, kq1;       // log2-domain logit of u = s (q . c) + m sum q
-  float o[4][4];
-  float m0, m1, l0, l1; // running maxima (shared by the lanes of a head), this lane's sums
-  float z0, z1;         // this lane's sum p m
-  float bound, inv;     // a power of two above every V scale so far, 2^15 / bound
+  float o[4][4];        // rows r + 8 hold sum w s (16 hi), rows r the sum of both halves
+  float m0, m1;         // running maxima rounded up to integers (NO_MAX: none yet), the same in a head's lanes
+  float bound, lift;    // a power of two above every V scale so far; log2(2^15 / bound)
+  uint64_t kq, nm;      // (kq0, kq1); (lift - m0, lift - m1): a weight is w = 2^(u kq + nm) = p 2^lift
+  uint64_t l;           // this lane's sums of w
+  float z0, z1;         // this lane's sums of w m
 };
 
-constexpr float MIN_BOUND = 7.888609052210118e-31f;   // 2^-100
+constexpr float NO_MAX = -1e30f;                      // below every logit that is not -inf
+constexpr float MIN_BOUND = 8.077935669463161e-28f;   // 2^-90: 2^lift stays far from fp32's end
 
 __device__ __forceinline__ void clear(Rows& s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) s.o[i][0] = s.o[i][1] = s.o[i][2] = s.o[i][3] = 0.f;
-  s.m0 = s.m1 = -INFINITY;
-  s.l0 = s.l1 = s.z0 = s.z1 = 0.f;
+  s.m0 = s.m1 = NO_MAX;
   s.bound = MIN_BOUND;
-  s.inv = 32768.f / MIN_BOUND;
+  s.lift = 105.f;
+  s.nm = pair(-NO_MAX, -NO_MAX);
+  s.l = pair(0.f, 0.f);
+  s.z0 = s.z1 = 0.f;
 }
 
 // The query operand of head g * 8 + r (q: its 64 values).
@@ -131,6 +169,7 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
   s.qs1 = __shfl_sync(0xffffffffu, qs, 8 * t + 4);
   s.kq0 = __shfl_sync(0xffffffffu, kq, 8 * t);
   s.kq1 = __shfl_sync(0xffffffffu, kq, 8 * t + 4);
+  s.kq = pair(s.kq0, s.kq1);
 }
 
 // Untiled bulk copy of `bytes` (a multiple of 16) into shared memory.
@@ -162,11 +201,12 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     const bool va = !TAIL || pg * P + 2 * r < ntok, vb2 = !TAIL || pg * P + 2 * r + 1 < ntok;
     if (!va) par.x = 0u;
     if (!vb2) par.y = 0u;
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_f16(c, w.x & LOW, w.z & LOW, w.x & HIGH, w.z & HIGH, s.qb[0][0], s.qb[0][1]);
-    mma_f16(c, (w.x >> 8) & LOW, (w.z >> 8) & LOW, (w.x >> 8) & HIGH, (w.z >> 8) & HIGH, s.qb[1][0], s.qb[1][1]);
+    float c[4];
+    mma_f16_zero(c, w.x & LOW, w.z & LOW, w.x & HIGH, w.z & HIGH, s.qb[0][0], s.qb[0][1]);
+    const uint32_t x8 = w.x >> 8, y8 = w.y >> 8, z8 = w.z >> 8, w8 = w.w >> 8;
+    mma_f16(c, x8 & LOW, z8 & LOW, x8 & HIGH, z8 & HIGH, s.qb[1][0], s.qb[1][1]);
     mma_f16(c, w.y & LOW, w.w & LOW, w.y & HIGH, w.w & HIGH, s.qb[2][0], s.qb[2][1]);
-    mma_f16(c, (w.y >> 8) & LOW, (w.w >> 8) & LOW, (w.y >> 8) & HIGH, (w.w >> 8) & HIGH, s.qb[3][0], s.qb[3][1]);
+    mma_f16(c, y8 & LOW, w8 & LOW, y8 & HIGH, w8 & HIGH, s.qb[3][0], s.qb[3][1]);
     const float sa = __uint_as_float(par.x << 16), ma = __uint_as_float(par.x & 0xffff0000u);
     const float sb = __uint_as_float(par.y << 16), mb = __uint_as_float(par.y & 0xffff0000u);
     u[pg][0] = va ? fmaf(sa, c[0], ma * s.qs0) : -INFINITY;
@@ -177,16 +217,15 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
   // V scales and minima, and what could move the running state: a logit above
   // its head's maximum, or a V scale at or above the bound.
   uint2 vp[PPW];
-  float x0 = fmaxf(u[0][0], u[0][2]), x1 = fmaxf(u[0][1], u[0][3]), top = 0.f;
+  float x0 = -INFINITY, x1 = -INFINITY, top = 0.f;
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     vp[pg] = *reinterpret_cast<const uint2*>(vb + pg * stride + CODE_BYTES + r * 8);
     if (TAIL && pg * P + 2 * r >= ntok) vp[pg].x = 0u;
     if (TAIL && pg * P + 2 * r + 1 >= ntok) vp[pg].y = 0u;
-    top = fmaxf(top, fmaxf(__uint_as_float(vp[pg].x << 16), __uint_as_float(vp[pg].y << 16)));
-    if (pg == 0) continue;
-    x0 = fmaxf(x0, fmaxf(u[pg][0], u[pg][2]));
-    x1 = fmaxf(x1, fmaxf(u[pg][1], u[pg][3]));
+    top = max3(top, __uint_as_float(vp[pg].x << 16), __uint_as_float(vp[pg].y << 16));
+    x0 = max3(x0, u[pg][0], u[pg][2]);
+    x1 = max3(x1, u[pg][1], u[pg][3]);
   }
   if (__any_sync(0xffffffffu, x0 * s.kq0 > s.m0 || x1 * s.kq1 > s.m1 || top >= s.bound)) {
 #pragma unroll
@@ -195,44 +234,44 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
       x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-    const float n0 = fmaxf(s.m0, x0 * s.kq0), n1 = fmaxf(s.m1, x1 * s.kq1);
-    const float a0 = n0 == -INFINITY ? 1.f : fast_exp2(s.m0 - n0), a1 = n1 == -INFINITY ? 1.f : fast_exp2(s.m1 - n1);
-    s.m0 = n0;
-    s.m1 = n1;
-    s.l0 *= a0;
-    s.l1 *= a1;
-    s.z0 *= a0;
-    s.z1 *= a1;
+    const float n0 = fmaxf(s.m0, ceilf(x0 * s.kq0)), n1 = fmaxf(s.m1, ceilf(x1 * s.kq1));
     float f = 1.f;
     if (top >= s.bound) {   // the same for every lane
       const float nb = pow2_bits(min(static_cast<int>(__float_as_uint(top) >> 23) + 1, 253));
       f = s.bound * (1.f / nb);
       s.bound = nb;
-      s.inv = 32768.f / nb;
+      s.lift = static_cast<float>(15 + 127 - static_cast<int>(__float_as_uint(nb) >> 23));
     }
+    const float a0 = fast_exp2(s.m0 - n0) * f, a1 = fast_exp2(s.m1 - n1) * f;
+    s.m0 = n0;
+    s.m1 = n1;
+    s.nm = pair(s.lift - n0, s.lift - n1);
+    float l0, l1;
+    split(s.l, l0, l1);
+    s.l = pair(l0 * a0, l1 * a1);
+    s.z0 *= a0;
+    s.z1 *= a1;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      s.o[q][0] *= a0 * f;
-      s.o[q][1] *= a1 * f;
-      s.o[q][2] *= a0 * f;
-      s.o[q][3] *= a1 * f;
+      s.o[q][0] *= a0;
+      s.o[q][1] *= a1;
+      s.o[q][2] *= a0;
+      s.o[q][3] *= a1;
     }
   }
-  const float b0 = s.m0 == -INFINITY ? 0.f : s.m0, b1 = s.m1 == -INFINITY ? 0.f : s.m1;
   float mass[2 * PPW];   // MODE SUM: this lane's share of the pages' masses, heads 2t and 2t + 1
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     float e[4];
-    e[0] = fast_exp2(fmaf(u[pg][0], s.kq0, -b0));
-    e[1] = fast_exp2(fmaf(u[pg][1], s.kq1, -b1));
-    e[2] = fast_exp2(fmaf(u[pg][2], s.kq0, -b0));
-    e[3] = fast_exp2(fmaf(u[pg][3], s.kq1, -b1));
-    mass[2 * pg] = e[0] + e[2];
-    mass[2 * pg + 1] = e[1] + e[3];
-    s.l0 += mass[2 * pg];
-    s.l1 += mass[2 * pg + 1];
-    const float sa = __uint_as_float(vp[pg].x << 16) * s.inv, ma = __uint_as_float(vp[pg].x & 0xffff0000u);
-    const float sb = __uint_as_float(vp[pg].y << 16) * s.inv, mb = __uint_as_float(vp[pg].y & 0xffff0000u);
+    split(fma2(pair(u[pg][0], u[pg][1]), s.kq, s.nm), e[0], e[1]);
+    split(fma2(pair(u[pg][2], u[pg][3]), s.kq, s.nm), e[2], e[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = fast_exp2(e[i]);
+    const uint64_t both = add2(pair(e[0], e[1]), pair(e[2], e[3]));
+    s.l = add2(s.l, both);
+    if (MODE == CE_MODE_SUM) split(both, mass[2 * pg], mass[2 * pg + 1]);
+    const float sa = __uint_as_float(vp[pg].x << 16), ma = __uint_as_float(vp[pg].x & 0xffff0000u);
+    const float sb = __uint_as_float(vp[pg].y << 16), mb = __uint_as_float(vp[pg].y & 0xffff0000u);
     s.z0 = fmaf(e[0], ma, fmaf(e[2], mb, s.z0));
     s.z1 = fmaf(e[1], ma, fmaf(e[3], mb, s.z1));
     const uint32_t p0 = movmatrix_trans(pack_f16(e[0] * sa, e[1] * sa));
@@ -240,8 +279,12 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     const uint4 w = *reinterpret_cast<const uint4*>(vb + pg * stride + (t * 8 + r) * 16);
     const uint32_t wq[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      mma_f16(s.o[q], wq[q] & LOW, wq[q] & HIGH, (wq[q] >> 8) & LOW, (wq[q] >> 8) & HIGH, p0, p1);
+    for (int q = 0; q < 4; ++q) {
+      // rows r take a byte's both codes, lo + 16 hi, rows r + 8 its 16 hi alone:
+      // finish() subtracts (the weights are the same, so exactly up to fp32)
+      const uint32_t even = __byte_perm(wq[q], 0u, 0x4240), odd = __byte_perm(wq[q], 0u, 0x4341);
+      mma_f16(s.o[q], even, even & HIGH, odd, odd & HIGH, p0, p1);
+    }
     if (MODE == CE_MODE_MAX) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -255,7 +298,7 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
   if (MODE == CE_MODE_SUM) {
     // Sum the 4 (page, head) shares over the lanes of equal t; each step halves
     // what a lane still carries, and lanes (r, t) of equal r / 2 end with page
-    // r / 4, head 2t + r / 2 % 2, whose log2 mass under the running maximum they keep.
+    // r / 4, head 2t + r / 2 % 2, whose log2 mass they keep.
     static_assert(PPW == 2, "four shares over eight lanes");
     float h2[2];
 #pragma unroll
@@ -267,35 +310,65 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     float y = mine + __shfl_xor_sync(0xffffffffu, yours, 8);
     y += __shfl_xor_sync(0xffffffffu, y, 4);
     const int pg = r >> 2, h = (r >> 1) & 1;
-    if (!(r & 1) && (!TAIL || pg * P < ntok) && side.cpos + pg < side.capacity)
-      side.ul[(side.cpos + pg) * side.H + side.hcol + h] = y > 0.f ? (h ? b1 : b0) + __log2f(y) : -INFINITY;
+    if (!(r & 1) && (!TAIL || pg * P < ntok) && side.cpos + pg < side.capacity) {
+      float n0, n1;
+      split(s.nm, n0, n1);
+      side.ul[(side.cpos + pg) * side.H + side.hcol + h] = y > 0.f ? __log2f(y) - (h ? n1 : n0) : -INFINITY;
+    }
+  }
+}
+
+// A warp's WT tokens of a stage, of which `mine` are left in the sequence.
+template <int WT, int stride, int MODE>
+__device__ __forceinline__ void stage(Rows& s, const uint8_t* kb, const uint8_t* vb, int mine, int lane, Side side) {
+  constexpr int STEP = PPW * P;
+  if (mine >= WT) {
+#pragma unroll 1
+    for (int i = 0; i < WT / STEP; ++i) {
+      tile<stride, false, MODE>(s, kb + i * PPW * stride, vb + i * PPW * stride, STEP, lane, side);
+      side.cpos += PPW;
+    }
+    return;
+  }
+#pragma unroll 1
+  for (; mine > 0; mine -= STEP) {
+    tile<stride, true, MODE>(s, kb, vb, mine, lane, side);
+    kb += PPW * stride;
+    vb += PPW * stride;
+    side.cpos += PPW;
   }
 }
 
 // The warp's sums over its lanes, and its output row in place: head 2t of dims
 // 16 q + r (i = 0) and 16 q + r + 8 (i = 2), head 2t + 1 likewise (i = 1, 3).
-__device__ __forceinline__ void finish(Rows& s) {
+__device__ __forceinline__ void finish(Rows& s, float& l0, float& l1) {
+  // sums hold w = p 2^lift; the accumulators w s (c 2^-24), upper nibbles 16-fold
+  const float down = pow2_bits(127 - static_cast<int>(s.lift));
+  split(s.l, l0, l1);
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
-    s.l0 += __shfl_xor_sync(0xffffffffu, s.l0, o);
-    s.l1 += __shfl_xor_sync(0xffffffffu, s.l1, o);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     s.z0 += __shfl_xor_sync(0xffffffffu, s.z0, o);
     s.z1 += __shfl_xor_sync(0xffffffffu, s.z1, o);
   }
-  // accumulators hold sum (p s 2^15 / bound) (c 2^-24), upper nibbles 16-fold;
-  // bound 2^9 in two steps that cannot overflow
-  const float fb = s.bound * 9.5367431640625e-7f;   // 2^-20
+  l0 *= down;
+  l1 *= down;
+  s.z0 *= down;
+  s.z1 *= down;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    s.o[q][0] = fmaf(s.o[q][0] * 536870912.f, fb, s.z0);
-    s.o[q][1] = fmaf(s.o[q][1] * 536870912.f, fb, s.z1);
-    s.o[q][2] = fmaf(s.o[q][2] * 33554432.f, fb, s.z0);
-    s.o[q][3] = fmaf(s.o[q][3] * 33554432.f, fb, s.z1);
+    s.o[q][0] = fmaf((s.o[q][0] - s.o[q][2]) * 16777216.f, down, s.z0);
+    s.o[q][1] = fmaf((s.o[q][1] - s.o[q][3]) * 16777216.f, down, s.z1);
+    s.o[q][2] = fmaf(s.o[q][2] * 1048576.f, down, s.z0);
+    s.o[q][3] = fmaf(s.o[q][3] * 1048576.f, down, s.z1);
   }
+  if (s.m0 == NO_MAX) s.m0 = -INFINITY;
+  if (s.m1 == NO_MAX) s.m1 = -INFINITY;
 }
 
 // A warp's heads into rows h0 .. h0 + 7 of a record-shaped buffer of H heads.
-__device__ __forceinline__ void put(const Rows& s, float* rec, int H, int h0, int lane) {
+__device__ __forceinline__ void put(const Rows& s, float l0, float l1, float* rec, int H, int h0, int lane) {
   const int r = lane >> 2, t = lane & 3;
   float* o = rec + (h0 + 2 * t) * D + r;
 #pragma unroll
@@ -308,9 +381,9 @@ __device__ __forceinline__ void put(const Rows& s, float* rec, int H, int h0, in
   if (r == 0) {
     float* ml = rec + H * D + (h0 + 2 * t) * 2;
     ml[0] = s.m0;
-    ml[1] = s.l0;
+    ml[1] = l0;
     ml[2] = s.m1;
-    ml[3] = s.l1;
+    ml[3] = l1;
   }
 }
 
@@ -323,13 +396,14 @@ template <int G>
 __device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp, int lane, float* part) {
   constexpr int H = G * GROUP, SUB = NW / G;
   float* rec = p.rec + static_cast<int64_t>(b + blockIdx.x) * rec_floats(H);
-  finish(s);
+  float l0, l1;
+  finish(s, l0, l1);
   if constexpr (SUB == 1) {
-    put(s, rec, H, warp * GROUP, lane);
+    put(s, l0, l1, rec, H, warp * GROUP, lane);
     return;
   }
   consumers_sync();   // the buffer is free (all warps leave the same sequences in the same order)
-  put(s, part + (warp / G) * rec_floats(H), H, (warp % G) * GROUP, lane);
+  put(s, l0, l1, part + (warp / G) * rec_floats(H), H, (warp % G) * GROUP, lane);
   consumers_sync();
   for (int i = threadIdx.x; i < H * D / 2; i += NW * 32) {
     const int h = i / (D / 2);
@@ -404,6 +478,16 @@ struct Shape {
   static_assert(CTAS_PER_SM * (SMEM + 2048) <= 228 * 1024, "two CTAs per SM");
 };
 
+template <int M>
+struct Mode {
+  static constexpr int value = M;
+};
+struct Ring {   // a consumer's place in the stage ring
+  int slot;
+  uint32_t phase;
+  bool aborted;
+};
+
 __device__ __forceinline__ int stages_of(const Params& p, int b, int ST) {
   return (decode::seq_tokens(p, b, P) + ST - 1) / ST;
 }
@@ -446,7 +530,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   int64_t S = 0;
   const int64_t excl = decode::block_excl_scan(local, scan_sh, S);   // a barrier: start_sh is set
   const int64_t k = blockIdx.x, grid = decode::eff_grid(S, gridDim.x, MIN_STAGES_LOG2);
-  const int64_t S_lo = k < grid ? k * S / grid : S, S_hi = k < grid ? (k + 1) * S / grid : S;
+  const int S_lo = static_cast<int>(k < grid ? k * S / grid : S);
+  const int S_hi = static_cast<int>(k < grid ? (k + 1) * S / grid : S);
   if (S_lo < S_hi && excl <= S_lo && S_lo < excl + local) {
     int64_t run = excl;
     for (int b = lo_b; b < hi_b; ++b) {
@@ -490,13 +575,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     };
     int64_t w0 = -1;
     int idx_cur = -2, idx_next = -2, idx_ahead = -2;
-    for (int64_t x = S_lo; x < S_hi; ++x, ++issued) {
+    for (int x = S_lo; x < S_hi; ++x, ++issued) {
       while (x >= base + nst) {
         base += nst;
         ++b;
         load_seq(b);
       }
-      const int j = static_cast<int>(x - base);
+      const int j = x - base;
       const int ntok = min(ST, tok_b - j * ST);
       const int nunits = (ntok + P - 1) / P;
       const int64_t c0 = ip_b + static_cast<int64_t>(j) * UPS;
@@ -547,67 +632,67 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     // ------------------------------- consumers -------------------------------
     const int g = warp % G, tb = warp / G;
     const int head = g * GROUP + (lane >> 2);
+    const uint8_t* mine0 = smem + tb * (WT / P) * UNIT_BYTES + g * SLICE;
     Rows st;
-    Side side{0, p.kv_capacity, H, g * GROUP + 2 * (lane & 3), p.ul, p.tl};
-    int cur_b = -1, mode = CE_MODE_NONE, s = 0;
-    uint32_t ph = 0;
-    bool aborted = false;
-    for (int64_t x = S_lo; x < S_hi; ++x) {
+    Ring ring{0, 0u, false};
+    // After a timeout a warp keeps walking (so that leave()'s barriers and the
+    // records stay in step) but waits for and computes nothing more.
+    auto begin = [&]() -> const uint8_t* {
+      if (!ring.aborted && !mbar_wait_or_abort(&full[ring.slot], ring.phase, p.err, abort_flag)) {
+        *abort_flag = 1;
+        ring.aborted = true;
+      }
+      return mine0 + ring.slot * STAGE_BYTES;
+    };
+    auto end = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[ring.slot]);   // release orders the reads above
+      if (++ring.slot == NSTAGES) {
+        ring.slot = 0;
+        ring.phase ^= 1u;
+      }
+    };
+    for (int x = S_lo; x < S_hi;) {
       while (x >= base + nst) {
         base += nst;
         ++b;
         load_seq(b);
       }
-      if (b != cur_b) {
-        if (cur_b >= 0) leave<G>(p, st, cur_b, warp, lane, part);
-        cur_b = b;
-        clear(st);
-        load_query(st, p.q + static_cast<int64_t>(b) * p.q_sb + static_cast<int64_t>(head) * p.q_sh, lane & 3,
-                   p.scale_log2);
-        mode = decode::seq_mode(p, b);
-        if ((mode == CE_MODE_SUM && !p.ul) || (mode == CE_MODE_MAX && !p.tl)) {
-          if (lane == 0 && warp == 0) flag_error(p.err, CE_EW_MODE);
-          mode = CE_MODE_NONE;
+      clear(st);
+      load_query(st, p.q + static_cast<int64_t>(b) * p.q_sb + static_cast<int64_t>(head) * p.q_sh, lane & 3,
+                 p.scale_log2);
+      int mode = decode::seq_mode(p, b);
+      if ((mode == CE_MODE_SUM && !p.ul) || (mode == CE_MODE_MAX && !p.tl)) {
+        if (lane == 0 && warp == 0) flag_error(p.err, CE_EW_MODE);
+        mode = CE_MODE_NONE;
+      }
+      Side side{ip_b + static_cast<int64_t>(x - base) * UPS + tb * (WT / P), p.kv_capacity, H,
+                g * GROUP + 2 * (lane & 3), p.ul, p.tl};
+      const int stop = min(S_hi, base + nst), whole = min(stop, base + tok_b / ST);
+      auto whole_stages = [&](auto md) {
+        for (; x < whole; ++x) {
+          const uint8_t* kb = begin();
+          if (!ring.aborted) stage<WT, UNIT_BYTES, decltype(md)::value>(st, kb, kb + HALF_STAGE, WT, lane, side);
+          side.cpos += UPS;
+          end();
         }
-      }
-      const int j = static_cast<int>(x - base);
-      const int mine = tok_b - j * ST - tb * WT;   // tokens from this warp's first page on
-      const int cs = s;
-      const uint32_t cph = ph;
-      if (++s == NSTAGES) {
-        s = 0;
-        ph ^= 1u;
-      }
-      // After a timeout the warp keeps walking (so the record writes stay in
-      // step) but waits for and computes nothing more.
-      if (!aborted && !mbar_wait_or_abort(&full[cs], cph, p.err, abort_flag)) {
-        *abort_flag = 1;
-        aborted = true;
-      }
-      if (aborted) continue;
-      const uint8_t* kb = smem + cs * STAGE_BYTES + tb * (WT / P) * UNIT_BYTES + g * SLICE;
-      const uint8_t* vb = kb + HALF_STAGE;
-      side.cpos = ip_b + static_cast<int64_t>(j) * UPS + tb * (WT / P);
-      constexpr int STEP = PPW * P;
-#pragma unroll 1
-      for (int left = mine; left > max(mine - WT, 0); left -= STEP) {
-        if (left >= STEP) {
-          if (mode == CE_MODE_SUM) tile<UNIT_BYTES, false, CE_MODE_SUM>(st, kb, vb, STEP, lane, side);
-          else if (mode == CE_MODE_MAX) tile<UNIT_BYTES, false, CE_MODE_MAX>(st, kb, vb, STEP, lane, side);
-          else tile<UNIT_BYTES, false, CE_MODE_NONE>(st, kb, vb, STEP, lane, side);
-        } else {
-          if (mode == CE_MODE_SUM) tile<UNIT_BYTES, true, CE_MODE_SUM>(st, kb, vb, left, lane, side);
-          else if (mode == CE_MODE_MAX) tile<UNIT_BYTES, true, CE_MODE_MAX>(st, kb, vb, left, lane, side);
-          else tile<UNIT_BYTES, true, CE_MODE_NONE>(st, kb, vb, left, lane, side);
+      };
+      if (mode == CE_MODE_SUM) whole_stages(Mode<CE_MODE_SUM>{});
+      else if (mode == CE_MODE_MAX) whole_stages(Mode<CE_MODE_MAX>{});
+      else whole_stages(Mode<CE_MODE_NONE>{});
+      if (x < stop) {   // the sequence's last stage
+        const int left = tok_b - (x - base) * ST - tb * WT;   // tokens from this warp's first page on
+        const uint8_t *kb = begin(), *vb = kb + HALF_STAGE;
+        if (!ring.aborted) {
+          if (mode == CE_MODE_SUM) stage<WT, UNIT_BYTES, CE_MODE_SUM>(st, kb, vb, left, lane, side);
+          else if (mode == CE_MODE_MAX) stage<WT, UNIT_BYTES, CE_MODE_MAX>(st, kb, vb, left, lane, side);
+          else stage<WT, UNIT_BYTES, CE_MODE_NONE>(st, kb, vb, left, lane, side);
         }
-        kb += PPW * UNIT_BYTES;
-        vb += PPW * UNIT_BYTES;
-        side.cpos += PPW;
+        end();
+        ++x;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[cs]);   // release orders the reads above
+      leave<G>(p, st, b, warp, lane, part);
     }
-    if (cur_b >= 0) leave<G>(p, st, cur_b, warp, lane, part);
   }
   __syncthreads();
 }
@@ -716,72 +801,100 @@ __global__ void __launch_bounds__(CB_THREADS) combine_kernel(const Params p, int
 }
 
 // Page scores of the batch from the combine kernel's normalisers: scores[g, unit]
-// += SUM: sum_h 2^(page log-mass - L_h), MAX: sum_t 2^(max_h (s_t,h - L_h)).  Block
-// (x, b) takes every gridDim.x-th group of pages of row b, all KV heads at
-// once, so that neighbouring threads read neighbouring heads and pages.
+// += SUM: sum_h 2^(page log-mass - L_h), MAX: sum_t 2^(max_h (s_t,h - L_h)).  Every
+// warp takes SC_PAGES consecutive positions of the CSR, all KV heads at once,
+// whatever rows they belong to: neighbouring lanes read neighbouring heads,
+// and a long row's pages are spread as evenly as the others'.
 constexpr int SC_THREADS = 256;
+constexpr int SC_PAGES = 4;
 
 template <int G>
 __global__ void __launch_bounds__(SC_THREADS) score_kernel(const Params p) {
   constexpr int H = G * GROUP;
-  const int b = blockIdx.y;
-  const int mode = decode::seq_mode(p, b);
-  if ((mode != CE_MODE_SUM || !p.ul) && (mode != CE_MODE_MAX || !p.tl)) return;
-  const int tokens = decode::seq_tokens(p, b, P);
-  const int npages = (tokens + P - 1) / P;
-  const int64_t ip = p.kv_indptr[b];
-  const int fresh = p.zero_new && (tokens - 1) % P == 0 ? npages - 1 : -1;
-  const int lane = threadIdx.x & 31;
-  const int g = lane % G;
-  float L[GROUP];
-  {
-    const float4* l4 = reinterpret_cast<const float4*>(p.lse2 + static_cast<int64_t>(b) * H + g * GROUP);
-    const float4 x = l4[0], y = l4[1];
-    L[0] = x.x, L[1] = x.y, L[2] = x.z, L[3] = x.w, L[4] = y.x, L[5] = y.y, L[6] = y.z, L[7] = y.w;
-  }
+  static_assert(SC_PAGES * 8 <= 32, "a lane per (page, head)");
+  // lanes as token lanes x heads: TPL tokens each (at G = 1 the upper 16 lanes
+  // repeat the lower)
+  constexpr int LANES = 32 / G, TL = LANES < P ? LANES : P, TPL = P / TL;
+  const int lane = threadIdx.x & 31, g = lane % G, tl = (lane / G) % TL;
+  const int64_t end = min(static_cast<int64_t>(p.kv_indptr[p.bs]), p.kv_capacity);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (SC_THREADS / 32) * SC_PAGES;
   float* sc = p.scores + g * p.score_sg;
-  auto add = [&](int j, float mass) {
-    const int unit = p.kv_indices[ip + j];
-    if (unit < 0 || unit >= p.pool_units) return;   // flagged by the attention kernel
-    sc[unit] = j == fresh ? mass : sc[unit] + mass;
-  };
-  if (mode == CE_MODE_SUM) {
-    constexpr int PB = SC_THREADS / G;   // pages per block and round
-    for (int j = blockIdx.x * PB + threadIdx.x / G; j < npages; j += gridDim.x * PB) {
-      if (ip + j >= p.kv_capacity) break;
-      const float4* u4 = reinterpret_cast<const float4*>(p.ul + (ip + j) * H + g * GROUP);
-      const float4 x = u4[0], y = u4[1];
-      const float u[GROUP] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      float mass = 0.f;
-#pragma unroll
-      for (int r = 0; r < GROUP; ++r) mass += fast_exp2(u[r] - L[r]);
-      add(j, mass);
+  for (int64_t c0 = (static_cast<int64_t>(blockIdx.x) * (SC_THREADS / 32) + (threadIdx.x >> 5)) * SC_PAGES; c0 < end;
+       c0 += step) {
+    // The row of position c0, by 32-way search: kv_indptr[lo] <= c0 < kv_indptr[hi].
+    int lo = 0, hi = p.bs;
+    while (hi - lo > 1) {
+      const int part = (hi - lo + 31) / 32, at = lo + lane * part;
+      const unsigned below = __ballot_sync(0xffffffffu, at < hi && p.kv_indptr[at] <= c0);
+      const int last = max(0, 31 - __clz(static_cast<int>(below)));   // lane 0's holds unless c0 precedes the list
+      hi = min(hi, lo + (last + 1) * part);
+      lo += last * part;
     }
-    return;
-  }
-  // A warp's lanes are token lanes x heads: a page takes TL of them (one page
-  // per warp, two at G = 1), TPL tokens each.
-  constexpr int LANES = 32 / G, TL = LANES < P ? LANES : P, TPL = P / TL, PW = LANES / TL;
-  const int tl = (lane / G) % TL, pw = lane / (G * TL);
-  const int step = gridDim.x * (SC_THREADS / 32) * PW;
-  for (int j0 = (blockIdx.x * (SC_THREADS / 32) + (threadIdx.x >> 5)) * PW; j0 < npages; j0 += step) {
-    const int j = j0 + pw;
-    const bool in = j < npages && ip + j < p.kv_capacity;
-    float mass = 0.f;
-#pragma unroll
-    for (int i = 0; i < TPL; ++i) {
-      const int t = tl + i * TL;
-      if (in && j * P + t < tokens) {
-        const float4* u4 = reinterpret_cast<const float4*>(p.tl + ((ip + j) * P + t) * H + g * GROUP);
-        const float4 x = u4[0], y = u4[1];
-        const float top = fmaxf(fmaxf(fmaxf(x.x - L[0], x.y - L[1]), fmaxf(x.z - L[2], x.w - L[3])),
-                                fmaxf(fmaxf(y.x - L[4], y.y - L[5]), fmaxf(y.z - L[6], y.w - L[7])));
-        mass += fast_exp2(top);
+    // Lane i < SC_PAGES: the row of position c0 + i, the page's place in it,
+    // its valid tokens (0: nothing to score) and unit.
+    int row = lo, valid = 0, unit = -1;
+    bool fresh = false, sum = false;
+    if (lane < SC_PAGES && c0 + lane < end) {
+      const int c = static_cast<int>(c0) + lane;
+      unit = p.kv_indices[c];
+      while (row + 1 < p.bs && p.kv_indptr[row + 1] <= c) ++row;
+      const int start = p.kv_indptr[row], tokens = decode::seq_tokens(p, row, P), mode = decode::seq_mode(p, row);
+      const int j = c - start;
+      sum = mode == CE_MODE_SUM && p.ul;
+      // a unit outside the pool was flagged by the attention kernel
+      if (j >= 0 && unit >= 0 && unit < p.pool_units && (sum || (mode == CE_MODE_MAX && p.tl))) {
+        valid = max(0, min(P, tokens - j * P));
+        fresh = p.zero_new && j * P + 1 == tokens;
       }
     }
+    // SUM pages, one lane per (page, head)
+    {
+      const int i = min(lane / G, SC_PAGES - 1);
+      const int n = __shfl_sync(0xffffffffu, valid, i), b = __shfl_sync(0xffffffffu, row, i);
+      const int to = __shfl_sync(0xffffffffu, unit, i);
+      const bool is_sum = __shfl_sync(0xffffffffu, sum, i), first = __shfl_sync(0xffffffffu, fresh, i);
+      if (n > 0 && is_sum && lane < SC_PAGES * G) {
+        const float old = sc[to];
+        const float4* l4 = reinterpret_cast<const float4*>(p.lse2 + static_cast<int64_t>(b) * H + g * GROUP);
+        const float4* u4 = reinterpret_cast<const float4*>(p.ul + (c0 + i) * H + g * GROUP);
+        const float4 L = l4[0], M = l4[1], x = u4[0], y = u4[1];
+        const float mass =
+            ((fast_exp2(x.x - L.x) + fast_exp2(x.y - L.y)) + (fast_exp2(x.z - L.z) + fast_exp2(x.w - L.w))) +
+            ((fast_exp2(y.x - M.x) + fast_exp2(y.y - M.y)) + (fast_exp2(y.z - M.z) + fast_exp2(y.w - M.w)));
+        sc[to] = first ? mass : old + mass;
+      }
+    }
+    // MAX pages one after another, their tokens over the lanes
+    unsigned todo = __ballot_sync(0xffffffffu, valid > 0 && !sum);
+    while (todo) {
+      const int i = __ffs(static_cast<int>(todo)) - 1;
+      todo &= todo - 1;
+      const int n = __shfl_sync(0xffffffffu, valid, i), b = __shfl_sync(0xffffffffu, row, i);
+      const int to = __shfl_sync(0xffffffffu, unit, i);
+      const bool first = __shfl_sync(0xffffffffu, fresh, i);
+      const float4* l4 = reinterpret_cast<const float4*>(p.lse2 + static_cast<int64_t>(b) * H + g * GROUP);
+      const float4 L = l4[0], M = l4[1];
+      const float old = lane < G ? sc[to] : 0.f;
+      float4 x[TPL], y[TPL];
 #pragma unroll
-    for (int o = G; o < G * TL; o <<= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    if (in && tl == 0) add(j, mass);
+      for (int k = 0; k < TPL; ++k) {
+        const int t = min(tl + k * TL, n - 1);   // valid tokens only
+        const float4* u4 = reinterpret_cast<const float4*>(p.tl + ((c0 + i) * P + t) * H + g * GROUP);
+        x[k] = u4[0];
+        y[k] = u4[1];
+      }
+      float mass = 0.f;
+#pragma unroll
+      for (int k = 0; k < TPL; ++k) {
+        const float top =
+            fmaxf(fmaxf(fmaxf(x[k].x - L.x, x[k].y - L.y), fmaxf(x[k].z - L.z, x[k].w - L.w)),
+                  fmaxf(fmaxf(y[k].x - M.x, y[k].y - M.y), fmaxf(y[k].z - M.z, y[k].w - M.w)));
+        mass += tl + k * TL < n ? fast_exp2(top) : 0.f;
+      }
+#pragma unroll
+      for (int o = G; o < G * TL; o <<= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+      if (lane < G) sc[to] = first ? mass : old + mass;
+    }
   }
 }
 
@@ -801,11 +914,12 @@ int launch(const Params& p, const uint8_t* k_pool, const uint8_t* v_pool, int sm
     combine_kernel<H, 1><<<static_cast<unsigned>((pairs + 7) / 8), CB_THREADS, 0, st>>>(p, grid);
   if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_kv4_decode combine launch");
   if ((score_flags & CE_SCORE_DEFER) || !(score_flags & 3) || !p.mode_of_row) return CE_OK;
-  // The scores are a launch of their own over all pages, about four blocks per
-  // SM over the batch (a task per row and head, as inside the bf16 combine,
-  // left the longest row's pages to one block: 371 us instead of 214).
-  const int x = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((4LL * sms + p.bs - 1) / p.bs, 512)));
-  score_kernel<G><<<dim3(x, p.bs), SC_THREADS, 0, st>>>(p);
+  // The scores are a launch of their own over all pages (a task per row and
+  // head, as inside the bf16 combine, left the longest row's pages to one
+  // block: 371 us instead of 214 at 64 rows of 2K-32K tokens).
+  const int64_t warps = (p.kv_capacity + SC_PAGES - 1) / SC_PAGES;
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((warps + SC_THREADS / 32 - 1) / (SC_THREADS / 32), 16LL * sms));
+  score_kernel<G><<<static_cast<unsigned>(blocks), SC_THREADS, 0, st>>>(p);
   if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_kv4_decode score launch");
   return CE_OK;
 }
