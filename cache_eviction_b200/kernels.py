@@ -187,46 +187,104 @@ def decode_scores(kv_indptr, kv_indices, kv_tokens, pool_units, page_size, H, G,
     _count(1 if score_flags & 3 else 0)
 
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _bad(what: str):
+    raise ValueError(what)
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _on(device: torch.device, *tensors) -> None:
     """Every tensor given lies on `device` (a CUDA device)."""
-    _require(device.type == "cuda" and all(t is None or t.device == device for t in tensors),
-             f"every tensor must be on one CUDA device, here {device}")
+    idx = device.index if device.type == "cuda" else -1
+    for t in tensors:
+        if t is not None and (idx < 0 or t.get_device() != idx):
+            _bad(f"every tensor must be on one CUDA device, here {device}")
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(fn, name: str, device: torch.device, *args) -> None:
+    """fn(*args, stream) on `device`'s current stream, with `device` current."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        st = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, _raw_stream(index))
+    if st:
+        capi.check(st, name)
+
+
+def _bytes(fn, name: str, device: torch.device, *args) -> int:
+    """A workspace query on `device` (the sizes go by its multiprocessors)."""
+    if torch.cuda.current_device() == device.index:
+        need = fn(*args)
+    else:
+        with torch.cuda.device(device.index):
+            need = fn(*args)
+    if need < 0:
+        raise capi.CeError(f"{name} failed")
+    return need
 
 
 def _csr(kv_indptr, kv_indices, kv_tokens, bs: int) -> None:
     for t in (kv_indptr, kv_indices, kv_tokens):
-        _require(t.dtype == torch.int32 and t.is_contiguous(), "kv_indptr, kv_indices and kv_tokens must be dense int32")
-    _require(kv_indptr.numel() >= bs + 1 and kv_tokens.numel() >= bs, "kv_indptr or kv_tokens shorter than the batch")
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            _bad("kv_indptr, kv_indices and kv_tokens must be dense int32")
+    if kv_indptr.numel() < bs + 1 or kv_tokens.numel() < bs:
+        _bad("kv_indptr or kv_tokens shorter than the batch")
 
 
 def _sinks(sinks, H: int):
     if sinks is None:
         return None
-    _require(sinks.numel() == H, "sinks must hold one value per query head")
-    return sinks.to(torch.float32).contiguous()
+    if sinks.numel() != H:
+        _bad("sinks must hold one value per query head")
+    return sinks if sinks.dtype == torch.float32 and sinks.is_contiguous() else sinks.to(torch.float32).contiguous()
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t [.., 64] with 16-byte aligned rows: itself, or a dense copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(st % 8 == 0 for st in t.stride()[:-1]):
+    """t [a, b, 64] with 16-byte aligned rows: itself, or a dense copy."""
+    s0, s1, s2 = t.stride()
+    if t.numel() == 0 or (s2 == 1 and not (s0 | s1) & 7 and not t.data_ptr() & 15):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _workspace(need: int, given: Optional[torch.Tensor], device, what: str) -> torch.Tensor:
+def _queries(q: torch.Tensor, align: int) -> torch.Tensor:
+    """q [a, H, 64] bf16 with dense rows and strides of `align` elements: itself, or a dense copy."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16:
+        _bad("q must be bf16 [queries, query heads, 64]")
+    s0, s1, s2 = q.stride()
+    if q.numel() == 0 or (s2 == 1 and not (s0 | s1) & (align - 1) and not q.data_ptr() & (2 * align - 1)):
+        return q
+    return q.clone(memory_format=torch.contiguous_format)
+
+
+def _output(out, shape, device, *dtypes) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtypes[0], device=device)
+    if out.dtype not in dtypes or out.shape != shape or (out.numel() and out.stride(2) != 1):
+        _bad(f"out must be {' or '.join(map(str, dtypes))} {list(shape)} with dense rows")
+    return out
+
+
+def _lse(lse, n: int):
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.numel() != n):
+        _bad("lse must be dense fp32 [batch, query heads]")
+
+
+def _workspace(need: int, given: Optional[torch.Tensor], device) -> torch.Tensor:
     """The caller's workspace, or one from torch's allocator for this call
     alone, which is safe on any stream and inside a capture (a graph keeps it)."""
-    if need < 0:
-        raise capi.CeError(f"{what} failed")
     if given is None:
         return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-    _require(given.dtype == torch.uint8 and given.is_contiguous() and given.numel() >= need and given.device == device,
-             f"workspace must be a dense uint8 tensor of at least {need} bytes on {device}")
+    if given.dtype != torch.uint8 or not given.is_contiguous() or given.numel() < need or given.device != device:
+        _bad(f"workspace must be a dense uint8 tensor of at least {need} bytes on {device}")
     return given
 
 
@@ -236,11 +294,11 @@ def kv4_pool(units: int, kv_heads: int, device) -> torch.Tensor:
 
 
 def _kv4_pools(k_pool, v_pool):
-    for t in (k_pool, v_pool):
-        _require(t.dtype == torch.uint8 and t.dim() == 3 and t.is_contiguous() and t.shape == k_pool.shape
-                 and t.shape[2] == capi.CE_KV4_SLICE_BYTES,
-                 f"4-bit pools must be dense uint8 [units, kv_heads, {capi.CE_KV4_SLICE_BYTES}] of one shape")
-    return k_pool.shape[0], k_pool.shape[1]
+    shape = k_pool.shape
+    if (k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or len(shape) != 3 or v_pool.shape != shape
+            or shape[2] != capi.CE_KV4_SLICE_BYTES or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
+        _bad(f"4-bit pools must be dense uint8 [units, kv_heads, {capi.CE_KV4_SLICE_BYTES}] of one shape")
+    return shape[0], shape[1]
 
 
 def kv4_write(k, v, k_pool, v_pool, loc, err=None):
@@ -251,17 +309,18 @@ def kv4_write(k, v, k_pool, v_pool, loc, err=None):
     + position in the page, distinct, negative ones skipped."""
     lib = capi.load()
     units, G = _kv4_pools(k_pool, v_pool)
-    _require(k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.dim() == 3 and k.shape == v.shape
-             and tuple(k.shape[1:]) == (G, 64), f"k and v must be bf16 [tokens, {G}, 64]")
-    _require(loc.dtype == torch.int64 and loc.is_contiguous() and loc.numel() == k.shape[0],
-             "loc must hold one int64 slot per token")
-    _on(k_pool.device, k, v, v_pool, loc, err)
+    if (k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 3 or k.shape != v.shape
+            or k.shape[1] != G or k.shape[2] != 64):
+        _bad(f"k and v must be bf16 [tokens, {G}, 64]")
+    tokens = k.shape[0]
+    if loc.dtype != torch.int64 or not loc.is_contiguous() or loc.numel() != tokens:
+        _bad("loc must hold one int64 slot per token")
+    dev = k_pool.device
+    _on(dev, k, v, k_pool, v_pool, loc, err)
     k, v = _rows16(k), _rows16(v)
-    with torch.cuda.device(k_pool.device):
-        st = lib.ce_kv4_write(_p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(loc), k.shape[0], G,
-                              64, 16, _p(k_pool), _p(v_pool), units, _p(err), _stream(k_pool.device))
-    capi.check(st, "ce_kv4_write")
-    _count(1 if k.shape[0] else 0)
+    _call(lib.ce_kv4_write, "ce_kv4_write", dev, _at(k), k.stride(0), k.stride(1), _at(v), v.stride(0), v.stride(1),
+          _at(loc), tokens, G, 64, 16, _at(k_pool), _at(v_pool), units, _at(err))
+    _count(1 if tokens else 0)
 
 
 def kv4_read(k_pool, v_pool, units, k_out=None, v_out=None, err=None):
@@ -270,19 +329,23 @@ def kv4_read(k_pool, v_pool, units, k_out=None, v_out=None, err=None):
     aligned rows).  Pages of negative units are left as they are."""
     lib = capi.load()
     pool_units, G = _kv4_pools(k_pool, v_pool)
-    _require(units.dtype == torch.int32 and units.dim() == 1 and units.is_contiguous(), "units must be dense int32 [n]")
-    n = int(units.numel())
-    shape = (n, G, 16, 64)
-    k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pool.device) if k_out is None else k_out
-    v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pool.device) if v_out is None else v_out
+    if units.dtype != torch.int32 or units.dim() != 1 or not units.is_contiguous():
+        _bad("units must be dense int32 [n]")
+    n = units.numel()
+    dev = k_pool.device
+    shape = torch.Size((n, G, 16, 64))
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
     for t in (k_out, v_out):
-        _require(t.dtype == torch.bfloat16 and tuple(t.shape) == shape and (n == 0 or t.stride(3) == 1),
-                 f"outputs must be bf16 {list(shape)} with dense rows")
-    _on(k_pool.device, v_pool, units, k_out, v_out, err)
-    with torch.cuda.device(k_pool.device):
-        st = lib.ce_kv4_read(_p(k_pool), _p(v_pool), pool_units, _p(units), n, G, 64, 16, _p(k_out), *k_out.stride()[:3],
-                             _p(v_out), *v_out.stride()[:3], _p(err), _stream(k_pool.device))
-    capi.check(st, "ce_kv4_read")
+        if t.dtype != torch.bfloat16 or t.shape != shape or (n and t.stride(3) != 1):
+            _bad(f"outputs must be bf16 {list(shape)} with dense rows")
+    _on(dev, k_pool, v_pool, units, k_out, v_out, err)
+    ku, kg, kt, _ = k_out.stride()
+    vu, vg, vt, _ = v_out.stride()
+    _call(lib.ce_kv4_read, "ce_kv4_read", dev, _at(k_pool), _at(v_pool), pool_units, _at(units), n, G, 64, 16,
+          _at(k_out), ku, kg, kt, _at(v_out), vu, vg, vt, _at(err))
     _count(1 if n else 0)
     return k_out, v_out
 
@@ -303,48 +366,46 @@ def kv4_decode_attn_score(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, s
     leaves the page scores to decode_scores, from the workspace then given."""
     lib = capi.load()
     units, G = _kv4_pools(k_pool, v_pool)
-    _require(q.dim() == 3 and q.dtype == torch.bfloat16, "q must be bf16 [batch, query heads, 64]")
+    q = _queries(q, 2)
     bs, H, D = q.shape
     dev = q.device
     _csr(kv_indptr, kv_indices, kv_tokens, bs)
-    if q.numel() and (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 2 or q.data_ptr() % 4):
-        q = q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((bs, H, D), dtype=torch.bfloat16, device=dev) if out is None else out
-    _require(out.dtype == torch.bfloat16 and tuple(out.shape) == (bs, H, D) and (bs == 0 or out.stride(2) == 1),
-             "out must be bf16 of q's shape with dense rows")
-    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == bs * H),
-             "lse must be dense fp32 [batch, query heads]")
+    out = _output(out, q.shape, dev, torch.bfloat16)
+    _lse(lse, bs * H)
+    score_sg = 0
     if scores is not None:
-        _require(scores.dtype == torch.float32 and scores.dim() == 2 and scores.shape[0] == G
-                 and scores.shape[1] >= units and scores.stride(1) == 1, "scores must be fp32 [kv_heads, units]")
-    _require(mode_of_row is None or (mode_of_row.dtype == torch.int32 and mode_of_row.is_contiguous()),
-             "mode_of_row must be dense int32")
-    _require(rows is None or (rows.dtype == torch.int64 and rows.is_contiguous() and rows.numel() >= bs),
-             "rows must hold one int64 row per batch entry")
-    _require(mode_of_row is None or rows is not None or mode_of_row.numel() >= bs, "mode_of_row shorter than the batch")
-    _require(workspace is not None or not score_flags & capi.CE_SCORE_DEFER,
-             "deferred scores need the caller's workspace")
-    _on(dev, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, mode_of_row, rows, scores, out, lse, err)
+        if (scores.dtype != torch.float32 or scores.dim() != 2 or scores.shape[0] != G or scores.shape[1] < units
+                or scores.stride(1) != 1):
+            _bad("scores must be fp32 [kv_heads, units]")
+        score_sg = scores.stride(0) if G > 1 else max(units, 1)
+    if mode_of_row is not None and (mode_of_row.dtype != torch.int32 or not mode_of_row.is_contiguous()
+                                    or (rows is None and mode_of_row.numel() < bs)):
+        _bad("mode_of_row must be dense int32, one per row")
+    if rows is not None and (rows.dtype != torch.int64 or not rows.is_contiguous() or rows.numel() < bs):
+        _bad("rows must hold one int64 row per batch entry")
+    if workspace is None and score_flags & capi.CE_SCORE_DEFER:
+        _bad("deferred scores need the caller's workspace")
+    _on(dev, q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, mode_of_row, rows, scores, out, lse, err)
     sinks = _sinks(sinks, H)
     cap = kv_indices.numel()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib.ce_kv4_decode_workspace_bytes(bs, cap, H, G, score_flags), workspace, dev,
-                        "ce_kv4_decode_workspace_bytes")
-        st = lib.ce_kv4_decode_attn_score(
-            _p(q), q.stride(0), q.stride(1), _p(k_pool), _p(v_pool), units, _p(kv_indptr), _p(kv_indices),
-            _p(kv_tokens), cap, _p(sinks), _p(mode_of_row), _p(rows), float(sm_scale), bs, H, G, D, 16, _p(scores),
-            scores.stride(0) if scores is not None else 0, 1 if zero_new else 0, _p(out), out.stride(0), out.stride(1),
-            _p(lse), score_flags, _p(ws), ws.numel(), _p(err), _stream(dev))
-    capi.check(st, "ce_kv4_decode_attn_score")
-    _count(2 if bs else 0)
+    if scores is None or mode_of_row is None:
+        score_flags &= ~3          # nothing to score: no room for it either
+    need = _bytes(lib.ce_kv4_decode_workspace_bytes, "ce_kv4_decode_workspace_bytes", dev, bs, cap, H, G, score_flags)
+    ws = _workspace(need, workspace, dev)
+    _call(lib.ce_kv4_decode_attn_score, "ce_kv4_decode_attn_score", dev, _at(q), q.stride(0), q.stride(1), _at(k_pool),
+          _at(v_pool), units, _at(kv_indptr), _at(kv_indices), _at(kv_tokens), cap, _at(sinks), _at(mode_of_row),
+          _at(rows), sm_scale, bs, H, G, D, 16, _at(scores), score_sg, 1 if zero_new else 0, _at(out), out.stride(0),
+          out.stride(1), _at(lse), score_flags, _at(ws), ws.numel(), _at(err))
+    _count((2 + (1 if score_flags & 3 and not score_flags & capi.CE_SCORE_DEFER else 0)) if bs else 0)
     return out
 
 
 def _bf16_pools(k_pool, v_pool, page_size):
-    for t in (k_pool, v_pool):
-        _require(t.dtype == torch.bfloat16 and t.dim() == 4 and t.is_contiguous() and t.shape == k_pool.shape
-                 and tuple(t.shape[2:]) == (page_size, 64), f"pools must be dense bf16 [units, kv_heads, {page_size}, 64]")
-    return k_pool.shape[0], k_pool.shape[1]
+    shape = k_pool.shape
+    if (k_pool.dtype != torch.bfloat16 or v_pool.dtype != torch.bfloat16 or len(shape) != 4 or v_pool.shape != shape
+            or shape[2] != page_size or shape[3] != 64 or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
+        _bad(f"pools must be dense bf16 [units, kv_heads, {page_size}, 64] of one shape")
+    return shape[0], shape[1]
 
 
 def window_decode(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sm_scale, page_size, window, first=0,
@@ -356,30 +417,21 @@ def window_decode(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sm_scale,
     Returns out [bs, H, 64] (bf16, or fp32 with out_f32)."""
     lib = capi.load()
     units, G = _bf16_pools(k_pool, v_pool, page_size)
-    _require(q.dim() == 3 and q.dtype == torch.bfloat16, "q must be bf16 [batch, query heads, 64]")
+    q = _queries(q, 2)
     bs, H, D = q.shape
     dev = q.device
     _csr(kv_indptr, kv_indices, kv_tokens, bs)
-    if q.numel() and (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 2 or q.data_ptr() % 4):
-        q = q.clone(memory_format=torch.contiguous_format)
-    if out is None:
-        out = torch.empty((bs, H, D), dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
-    _require(out.dtype in (torch.float32, torch.bfloat16) and tuple(out.shape) == (bs, H, D)
-             and (bs == 0 or out.stride(2) == 1), "out must be bf16 or fp32 of q's shape with dense rows")
-    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == bs * H),
-             "lse must be dense fp32 [batch, query heads]")
-    _on(dev, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, out, lse, err)
+    out = _output(out, q.shape, dev, *((torch.float32, torch.bfloat16) if out_f32 else (torch.bfloat16, torch.float32)))
+    _lse(lse, bs * H)
+    _on(dev, q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, out, lse, err)
     sinks = _sinks(sinks, H)
     cap = kv_indices.numel()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib.ce_decode_workspace_bytes(bs, cap, H, G, page_size, 0), workspace, dev,
-                        "ce_decode_workspace_bytes")
-        st = lib.ce_window_decode(
-            _p(q), q.stride(0), q.stride(1), _p(k_pool), _p(v_pool), units, _p(kv_indptr), _p(kv_indices),
-            _p(kv_tokens), cap, _p(sinks), float(sm_scale), bs, H, G, D, page_size, int(window), int(first), _p(out),
-            1 if out.dtype == torch.float32 else 0, out.stride(0), out.stride(1), _p(lse), _p(ws), ws.numel(), _p(err),
-            _stream(dev))
-    capi.check(st, "ce_window_decode")
+    need = _bytes(lib.ce_decode_workspace_bytes, "ce_decode_workspace_bytes", dev, bs, cap, H, G, page_size, 0)
+    ws = _workspace(need, workspace, dev)
+    _call(lib.ce_window_decode, "ce_window_decode", dev, _at(q), q.stride(0), q.stride(1), _at(k_pool), _at(v_pool),
+          units, _at(kv_indptr), _at(kv_indices), _at(kv_tokens), cap, _at(sinks), sm_scale, bs, H, G, D, page_size,
+          window, first, _at(out), 1 if out.dtype == torch.float32 else 0, out.stride(0), out.stride(1), _at(lse),
+          _at(ws), ws.numel(), _at(err))
     _count(2 if bs else 0)
     return out
 
@@ -393,28 +445,22 @@ def window_prefill(q, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_token
     out [total_q, H, 64] bf16; rows of no entry keep what they held."""
     lib = capi.load()
     units, G = _bf16_pools(k_pool, v_pool, page_size)
-    _require(q.dim() == 3 and q.dtype == torch.bfloat16, "q must be bf16 [queries, query heads, 64]")
+    q = _queries(q, 8)
     total_q, H, D = q.shape
-    bs = int(kv_tokens.numel())
+    if total_q and (q.stride(1) < D or q.stride(0) < H * q.stride(1)):
+        q = q.clone(memory_format=torch.contiguous_format)     # heads outside their token's row
+    bs = kv_tokens.numel()
     dev = q.device
     _csr(kv_indptr, kv_indices, kv_tokens, bs)
-    _require(qo_indptr.dtype == torch.int32 and qo_indptr.is_contiguous() and qo_indptr.numel() >= bs + 1,
-             "qo_indptr must hold one more dense int32 than there are entries")
-    if q.numel() and (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16
-                      or q.stride(1) < D or q.stride(0) < H * q.stride(1)):
-        q = q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((total_q, H, D), dtype=torch.bfloat16, device=dev) if out is None else out
-    _require(out.dtype == torch.bfloat16 and tuple(out.shape) == (total_q, H, D) and (total_q == 0 or out.stride(2) == 1),
-             "out must be bf16 of q's shape with dense rows")
-    _on(dev, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sinks, out, err)
+    if qo_indptr.dtype != torch.int32 or not qo_indptr.is_contiguous() or qo_indptr.numel() < bs + 1:
+        _bad("qo_indptr must hold one more dense int32 than there are entries")
+    out = _output(out, q.shape, dev, torch.bfloat16)
+    _on(dev, q, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sinks, out, err)
     sinks = _sinks(sinks, H)
-    with torch.cuda.device(dev):
-        st = lib.ce_window_prefill(
-            _p(q), q.stride(0), q.stride(1), _p(k_pool), _p(v_pool), units, _p(qo_indptr), _p(kv_indptr),
-            _p(kv_indices), _p(kv_tokens), kv_indices.numel(), _p(sinks), float(sm_scale), bs, H, G, D, page_size,
-            total_q, int(max_q), int(max_tokens), int(window), int(first), _p(out), out.stride(0), out.stride(1),
-            _p(err), _stream(dev))
-    capi.check(st, "ce_window_prefill")
+    _call(lib.ce_window_prefill, "ce_window_prefill", dev, _at(q), q.stride(0), q.stride(1), _at(k_pool), _at(v_pool),
+          units, _at(qo_indptr), _at(kv_indptr), _at(kv_indices), _at(kv_tokens), kv_indices.numel(), _at(sinks),
+          sm_scale, bs, H, G, D, page_size, total_q, max_q, max_tokens, window, first, _at(out), out.stride(0),
+          out.stride(1), _at(err))
     _count(1 if bs and max_q and total_q else 0)
     return out
 

@@ -59,16 +59,29 @@ def special_rows(T, G, gen):
 
 
 @pytest.mark.parametrize("T,G", [(1, 8), (3, 1), (16, 2), (17, 8), (64, 8), (257, 4), (1000, 3)])
-def test_write_then_read_is_the_format(T, G):
+@pytest.mark.parametrize("run", ["scattered", "run", "offset run", "two runs", "runs with padding"])
+def test_write_then_read_is_the_format(T, G, run):
     from cache_eviction_b200 import kernels
     gen = torch.Generator().manual_seed(T * 10 + G)
     units = -(-T // 16) + 5
     k, v = special_rows(T, G, gen), special_rows(T, G, gen).flip(2)
     pools = [ref.random_pool(units, G, key, gen) for key in (True, False)]
-    loc = torch.randperm(units * 16, generator=gen)[:T]
+    order = torch.randperm(units, generator=gen)
+    slots = (order[:, None] * 16 + torch.arange(16)).view(-1)      # consecutive positions of scattered units
+    if run == "scattered":
+        loc = torch.randperm(units * 16, generator=gen)[:T]
+    elif run == "two runs":
+        loc = torch.cat((slots[7:7 + T // 2], slots[units * 16 - (T - T // 2):]))
+    else:
+        loc = slots[(0 if run == "run" else 21):][:T].clone()
+    written = torch.ones(T, dtype=torch.bool)
+    if run == "runs with padding":
+        written[torch.randperm(T, generator=gen)[:T // 5]] = False
+        loc[~written] = -1
     dk, dv = pools[0].to(DEV), pools[1].to(DEV)
     err = torch.zeros(1, dtype=torch.int32, device=DEV)
     kernels.kv4_write(k.to(DEV), v.to(DEV), dk, dv, loc.to(DEV), err=err)
+    k, v, loc = k[written], v[written], loc[written]
     want = []
     for pool, x, key in ((pools[0], k, True), (pools[1], v, False)):
         c, s, m = ref.unpack(pool, key)
@@ -81,13 +94,36 @@ def test_write_then_read_is_the_format(T, G):
     for got, exp in ((dk.cpu(), want[0]), (dv.cpu(), want[1])):
         assert torch.equal(got[..., :512], exp[..., :512])
         assert same_bits(got[..., 512:].contiguous().view(torch.bfloat16), exp[..., 512:].contiguous().view(torch.bfloat16))
-    order = torch.randperm(units, generator=gen).to(torch.int32)
+    order = order.to(torch.int32)
     rk, rv = kernels.kv4_read(dk, dv, order.to(DEV), err=err)
     assert int(err.item()) == 0
     for got, exp, key in ((rk, want[0], True), (rv, want[1], False)):
         # m + c s is one rounding away from exact in 64 bits, then one to bf16
         x = ref.values(exp[order.long()], key).float().to(torch.bfloat16)
         assert same_bits(got.cpu(), x)
+
+
+def test_ties_round_to_even_codes():
+    """Rows on which every (x - m) / s is a multiple of 1/2 or 1/4, over many
+    scales: the codes are those of an IEEE division with ties to even."""
+    from cache_eviction_b200 import kernels
+    rows = []
+    for e in list(range(-130, 120, 5)) + [-133]:
+        for step in (1, 3, 5, 7, 129, 131, 255):
+            s = step * 2.0 ** e
+            for q in (2.0, 4.0):
+                x = torch.arange(64, dtype=torch.float64).remainder(15 * q + 1) / q * s
+                rows += [x, x - 7.5 * s, -x]
+    x = torch.stack(rows).clamp(-3.38e38, 3.38e38).to(torch.bfloat16).view(-1, 1, 64)
+    T = x.shape[0]
+    units = -(-T // 16)
+    pool = torch.zeros((2, units, 1, 576), dtype=torch.uint8, device=DEV)
+    kernels.kv4_write(x.to(DEV), x.to(DEV), pool[0], pool[1], torch.arange(T, device=DEV))
+    want = [t.view(-1, *t.shape[2:]) for t in ref.quantise(x)]
+    for kv, key in ((0, True), (1, False)):
+        got = [t.view(units * 16, -1)[:T] for t in ref.unpack(pool[kv].cpu()[:, 0], key)]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b.double().view(T, -1))
 
 
 def test_rounding_stays_within_half_a_step():
