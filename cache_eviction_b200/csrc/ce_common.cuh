@@ -94,6 +94,26 @@ __device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parit
   }
 }
 
+// The same for kernels whose warps wait most of the time: the abort flag and the
+// timer are looked at every 64 tries only, so that a waiting warp takes few
+// issue slots from the others.
+__device__ __forceinline__ bool mbar_wait_quiet(uint64_t* bar, uint32_t parity, int32_t* err, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  unsigned long long t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    const unsigned long long now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      flag_error(err, CE_EW_TIMEOUT);
+      return false;
+    }
+  }
+}
+
 // ---- TMA: 2D tiled bulk-tensor load into shared memory, no multicast --------
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tmap, int32_t x,
                                             int32_t y, uint64_t* bar) {
@@ -360,6 +380,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_
   return __shfl_sync(0xffffffffu, ok, 0);
 }
 
+// The same with mbar_wait_quiet.
+__device__ __forceinline__ bool warp_wait_quiet(uint64_t* bar, uint32_t parity, int32_t* err, volatile int* abort,
+                                                int lane) {
+  bool ok = true;
+  if (lane == 0) ok = mbar_wait_quiet(bar, parity, err, abort);
+  return __shfl_sync(0xffffffffu, ok, 0);
+}
+
 // ---- exponentials ------------------------------------------------------------------
 // 2^x with the SFU's approximate exp2 (PTX ex2.approx.ftz.f32): relative
 // error near 2^-22, -inf -> +0, results below the normal range flush to 0.
@@ -383,6 +411,38 @@ __device__ __forceinline__ float poly_exp2(float x) {
   const float f = x - (t - 12582912.f);
   const float p = fmaf(fmaf(fmaf(0.055174146f, f, 0.24261758f), f, 0.69326109f), f, 0.99992758f);
   return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
+}
+
+// ---- packed fp32 --------------------------------------------------------------------
+// Two fp32 in one 64-bit register, for the instructions that work on both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void split(uint64_t d, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// The largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 }  // namespace ce

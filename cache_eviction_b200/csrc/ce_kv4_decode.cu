@@ -74,31 +74,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
-// Pairs of fp32 in one 64-bit register, for the packed fp32 instructions.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void split(uint64_t d, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 __device__ __forceinline__ float pow2_bits(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 
@@ -597,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
         idx_ahead = fetch(w0 + 64);
       }
       const int s = issued % NSTAGES;
-      if (issued >= NSTAGES && !warp_wait(&empty[s], ((issued / NSTAGES) & 1) ^ 1, p.err, abort_flag, lane)) {
+      if (issued >= NSTAGES && !warp_wait_quiet(&empty[s], ((issued / NSTAGES) & 1) ^ 1, p.err, abort_flag, lane)) {
         *abort_flag = 1;
         break;
       }
@@ -638,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     // After a timeout a warp keeps walking (so that leave()'s barriers and the
     // records stay in step) but waits for and computes nothing more.
     auto begin = [&]() -> const uint8_t* {
-      if (!ring.aborted && !mbar_wait_or_abort(&full[ring.slot], ring.phase, p.err, abort_flag)) {
+      if (!ring.aborted && !mbar_wait_quiet(&full[ring.slot], ring.phase, p.err, abort_flag)) {
         *abort_flag = 1;
         ring.aborted = true;
       }

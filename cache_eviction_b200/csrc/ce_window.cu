@@ -5,31 +5,36 @@
 //   out_i = softmax over {t <= p, t > p - window or t < first} (and the sink) of
 //           scale q_i . k_t,  times v_t,    p = kv_tokens - nq + i
 //
-// One CTA per (16 queries, KV head, entry): its 128 accumulator rows are the
-// 16 queries' 8 heads, which share every key and value tile.  It walks the
-// 128-key tiles that hold a visible token of some row (the first tokens'
-// tiles, then the window's, which start at a page boundary), in one pass:
-//   load warp     K and V tiles in the order the MMA warp takes them, through
-//                 a ring of five 16 KB slots (page loads by TMA, or cp.async
-//                 gathers for pages under 8 tokens)
-//   MMA warp      S(t) = Q K^T into tensor memory, then O += P(t-1) V
-//   softmax warps one thread per row: S from tensor memory, running maximum
-//                 and sum, P = 2^(s - m) in bf16 back into tensor memory as the
-//                 A operand of the second product.  O is rescaled only when a
-//                 row's maximum has grown by more than 2^8 since the last
-//                 rescale (P stays below 2^8, its relative precision and the
-//                 fp32 sum's are the same), so S(t+1) and P V(t) run under
-//                 the exponentials of tile t.
-// Two CTAs share an SM (256 TMEM columns and 97 KB each), so that one's
-// exponentials cover the other's waits.  The exponentials bound the kernel:
-// one per (row, key) of a tile against 2 x 128 x 64 multiply-adds, so a share of
-// them runs as a polynomial on the FMA pipes.  P in bf16 is rounded by at most
-// 2^-9 of itself, less than the output's own rounding makes of it on average;
-// maxima, sums and O are fp32.
+// One CTA per (32 queries, KV head, entry), two tiles of 16 queries whose 8
+// heads are a tile's 128 accumulator rows and share every key and value tile.
+// It walks the 128-key tiles that hold a visible token of some row (the first
+// tokens' tiles, then the window's, which start at a page boundary), in one pass:
+//   load warps    K tiles through one ring of 16 KB slots, V tiles through
+//                 another (page loads by TMA, or cp.async gathers for pages
+//                 under 8 tokens), page indices read a tile ahead
+//   S warp        S(t) = Q K^T of both query tiles into tensor memory, each as
+//                 soon as its S(t-1) is read
+//   PV warp       O += P(t) V(t) of each once its weights are in place
+//   softmax warps eight per query tile, two threads per row, 64 keys each: S from
+//                 tensor memory, running maximum (exchanged through shared
+//                 memory) and sum, P = 2^(s - m) in bf16 back into tensor
+//                 memory as the A operand of the second product.  O is
+//                 rescaled only when a row's maximum has grown by more than
+//                 2^8 since the last rescale (P stays below 2^8, its relative
+//                 precision and the fp32 sum's are the same).
+// The exponentials bound the kernel (one per row and key on a unit of 16 per
+// clock and SM: 1,024 clocks per tile, against 768 of the tensor cores), so the
+// two query tiles take turns at them: while one computes its weights the
+// other's waits, reads and maxima go on.  Left to themselves (two CTAs per SM)
+// the tiles fell into step, both at the exponentials and then both waiting.
+// (Taking a share of the exponentials as a polynomial on the FMA pipes was
+// slower at every share.)  P in bf16 is rounded by at most 2^-9 of itself, less
+// than the output's own rounding makes of it on average; maxima, sums and O
+// are fp32.
 //
 // What a row must not see must not reach it: a masked key's logit is replaced
 // before the maximum, and a masked value meets P = 0, which is no help if it
-// is infinite or NaN.  So in a tile that some row sees only in part the MMA
+// is infinite or NaN.  So in a tile that some row sees only in part the PV
 // warp clears the values that no row sees (a page's unwritten slots, pages that
 // were not loaded) and any value that is not finite, noting its token; a row
 // that does see such a token gets NaN at the end.
@@ -47,14 +52,16 @@ constexpr int GROUP = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int BM = 128;                  // accumulator rows
 constexpr int BN = 128;                  // keys per tile
-constexpr int QT = BM / GROUP;           // 16 queries per CTA
+constexpr int QT = BM / GROUP;           // 16 queries per tile
+constexpr int TILES = 2;                 // query tiles per CTA
 constexpr int TILE = 128 * 128;          // 128 rows x 128 B
-constexpr int SLOTS = 5;                 // ring of K and V tiles
+constexpr int KS = 5, VS = 5;            // ring slots of K and V tiles
 constexpr int LAG = 3;                   // cp.async tiles in flight before one is published
-constexpr int SM_WARPS = 4;              // softmax: TMEM lanes 32 w .. +31
-constexpr int LOAD_WARP = SM_WARPS, MMA_WARP = SM_WARPS + 1;
-constexpr int THREADS = 32 * (SM_WARPS + 2);
-constexpr uint32_t TMEM_COLS = 256, P_COL = 128, O_COL = 192;
+constexpr int SM_WARPS = 8;              // softmax, per query tile: TMEM lanes 32 (w % 4) .. +31, keys 64 (w / 4) .. +63
+constexpr int HALF = BN / 2;             // keys of a softmax thread
+constexpr int K_WARP = TILES * SM_WARPS, V_WARP = K_WARP + 1, S_WARP = K_WARP + 2;   // and the PV warp
+constexpr int THREADS = 32 * (TILES * SM_WARPS + 4);
+constexpr uint32_t TMEM_TILE = 256, TMEM_COLS = TILES * TMEM_TILE, P_COL = 128, O_COL = 192;   // S | P | O of each tile
 constexpr uint32_t IDESC_S = f16_idesc(BM, BN);
 constexpr uint32_t IDESC_PV = f16_idesc(BM, D) | kIdescBMajorMN;
 constexpr float LAZY = 8.f;              // log2 growth of a maximum that is let through
@@ -76,12 +83,13 @@ struct Params {
 };
 
 struct Sync {
-  uint64_t full[SLOTS], empty[SLOTS];
-  uint64_t sfull, sempty, pfull, pempty;
-  uint64_t once, odone, mma_done;
+  uint64_t kfull[KS], kempty[KS], vfull[VS], vempty[VS];
+  uint64_t sfull[TILES], sempty[TILES], pfull[TILES], pempty[TILES];
+  uint64_t once, odone, s_done, pv_done;
   uint32_t tmem;
   int abort;
-  int edges;                      // tiles whose values the MMA warp looked through
+  float top[TILES][2][2][BM];     // by query tile, key tile parity and half: the rows' maxima; at the end their sums
+  int edges;                      // tiles in whose values the PV warp found some that are not finite
   int edge_key[MAX_EDGE];         // their first token
   uint32_t edge_bad[MAX_EDGE][4]; // their tokens with a value that is not finite
 };
@@ -128,44 +136,81 @@ __device__ __forceinline__ bool entry_ok(const Params& p, int b, int& qbeg, int&
   return ok;
 }
 
-// Unit of the list's token t, or -1 (outside the pool: flagged).
-__device__ __forceinline__ int token_unit(const Params& p, int list0, int t) {
-  const int unit = p.kv_indices[list0 + t / p.P];
-  if (unit >= 0 && unit < p.pool_units) return unit;
-  flag_error(p.err, CE_EW_INDEX);
-  return -1;
-}
-
-// Keys k0 .. k0 + 127 of head g by page loads (pages of at least 8 rows, each
-// on a 1024-byte boundary of the tile), completing on `bar`.
-__device__ __forceinline__ void tma_tile(const Params& p, const Span& sp, const CUtensorMap* map, uint8_t* tile,
-                                         uint64_t* bar, int list0, int k0, int g, int lane) {
-  const int t = k0 + lane * p.P;
-  const int unit = lane < BN / p.P && sp.some(t, p.P) ? token_unit(p, list0, t) : -1;
-  const unsigned valid = __ballot_sync(0xffffffffu, unit >= 0);
-  if (lane == 0) mbar_arrive_expect_tx(bar, __popc(valid) * p.P * 128);
-  __syncwarp();
-  if (unit >= 0) tma_load_2d(tile + lane * p.P * 128, map, 0, (unit * p.G + g) * p.P, bar);
-}
-
-// The same for smaller pages by cp.async; rows that no query sees are zeros.
-__device__ __forceinline__ void copy_tile(const Params& p, const Span& sp, const __nv_bfloat16* pool, uint32_t tile,
-                                          int list0, int k0, int g, int lane) {
-  int u[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int t = k0 + lane + 32 * k;
-    u[k] = sp.some(t, 1) ? token_unit(p, list0, t) : -1;
+// A load warp's tiles of one pool through its ring.  PAGE: tokens per page, or
+// 0 for any size that divides 64.
+template <int PAGE, int SLOTS>
+__device__ __forceinline__ void load_tiles(const Params& p, const Span& sp, const CUtensorMap* map,
+                                           const __nv_bfloat16* pool, uint8_t* ring, uint64_t* full, uint64_t* empty,
+                                           int list0, int g, int lane, volatile int* abort) {
+  const int P = PAGE ? PAGE : p.P;
+  const bool tma = P >= 8;
+  // Pages of at least 8 rows: lane i < 128 / P the tile's page i.  Smaller ones:
+  // lane i keys i, i + 32, i + 64 and i + 96.
+  auto unit_of = [&](int k) -> int {   // unit holding key k, -1 if no row sees it
+    return sp.some(k, tma ? P : 1) ? p.kv_indices[list0 + k / P] : -1;
+  };
+  auto checked = [&](int unit, int k) -> int {
+    if (unit >= 0 && unit < p.pool_units) return unit;
+    if (sp.some(k, tma ? P : 1)) flag_error(p.err, CE_EW_INDEX);
+    return -1;
+  };
+  int t = 0;
+  if (tma) {
+    const int pages = BN / P;
+    int next = lane < pages ? unit_of(sp.key(0) + lane * P) : -1;
+    for (; t < sp.ntiles; ++t) {
+      const int s = t % SLOTS, k0 = sp.key(t) + lane * P;
+      const int unit = lane < pages ? checked(next, k0) : -1;
+      if (t + 1 < sp.ntiles) next = lane < pages ? unit_of(sp.key(t + 1) + lane * P) : -1;
+      const unsigned valid = __ballot_sync(0xffffffffu, unit >= 0);
+      if (t >= SLOTS && !warp_wait_quiet(&empty[s], ((t / SLOTS) & 1) ^ 1, p.err, abort, lane)) {
+        *abort = 1;
+        break;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(valid) * P * 128);
+      __syncwarp();
+      if (unit >= 0) tma_load_2d(ring + s * TILE + lane * P * 128, map, 0, (unit * p.G + g) * P, &full[s]);
+    }
+    if (lane == 0)   // every issued load lands before the CTA may exit
+      for (int u = max(0, t - SLOTS); u < t; ++u) mbar_wait(&full[u % SLOTS], (u / SLOTS) & 1, p.err);
+    return;
   }
-  const int c = lane & 7;
-#pragma unroll
-  for (int j = 0; j < BN / 4; ++j) {
-    const int r = (lane >> 3) + 4 * j;
-    const int unit = __shfl_sync(0xffffffffu, u[j >> 3], r & 31);
-    const bool ok = unit >= 0;
-    const __nv_bfloat16* src =
-        ok ? pool + ((static_cast<int64_t>(unit) * p.G + g) * p.P + (k0 + r) % p.P) * D + c * 8 : pool;
-    cp_async16(tile + swz(r, c), src, ok);
+  if constexpr (PAGE == 0) {
+    for (; t < sp.ntiles; ++t) {
+      const int s = t % SLOTS, k0 = sp.key(t);
+      int u[4];
+  #pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = unit_of(k0 + lane + 32 * i);
+  #pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = checked(u[i], k0 + lane + 32 * i);
+      if (t >= SLOTS && !warp_wait_quiet(&empty[s], ((t / SLOTS) & 1) ^ 1, p.err, abort, lane)) {
+        *abort = 1;
+        break;
+      }
+      const int c = lane & 7;
+  #pragma unroll 4
+      for (int j = 0; j < BN / 4; ++j) {
+        const int r = (lane >> 3) + 4 * j;
+        const int from = (j >> 3) == 0 ? u[0] : (j >> 3) == 1 ? u[1] : (j >> 3) == 2 ? u[2] : u[3];
+        const int unit = __shfl_sync(0xffffffffu, from, r & 31);
+        const bool ok = unit >= 0;   // rows that no query sees are zeros
+        const __nv_bfloat16* src =
+            ok ? pool + ((static_cast<int64_t>(unit) * p.G + g) * P + (k0 + r) % P) * D + c * 8 : pool;
+        cp_async16(smem_addr(ring) + s * TILE + swz(r, c), src, ok);
+      }
+      cp_async_commit();
+      if (t >= LAG) {
+        cp_async_wait<LAG>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[(t - LAG) % SLOTS]);
+      }
+    }
+    cp_async_wait<0>();
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0 && !*abort)
+      for (int u = max(0, t - LAG); u < t; ++u) mbar_arrive(&full[u % SLOTS]);
   }
 }
 
@@ -174,261 +219,302 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
 
-// A partly visible value tile (keys from k on) made safe for P = 0 (one warp).
+// 0 * w added to acc, per half: NaN from the first value that is not finite on.
+__device__ __forceinline__ uint32_t taint(uint32_t w, uint32_t acc) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(acc));
+  return d;
+}
+
+// A partly visible value tile (keys from k on) made safe for P = 0, by one warp:
+// rows that no query sees are cleared, then values that are not finite, whose
+// tokens are noted.
 __device__ __forceinline__ void clean_values(const Span& sp, uint8_t* tile, int k, Sync* sy, int lane) {
   const int e = sy->edges;
   __syncwarp();
-  uint32_t bad[4] = {0u, 0u, 0u, 0u};
+  uint8_t* mine = tile + (lane >> 3) * 128 + (lane & 7) * 16;
+  const int row0 = lane >> 3, end = sp.p_hi + 1 - k, from = sp.lo - k, head = sp.first - k;
+  uint32_t acc[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int i0 = 0; i0 < BN / 4; i0 += 8) {
+    uint4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(mine + (i0 + i) * 512);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = w * 32 + i * 4 + (lane >> 3);
-      uint4* at = reinterpret_cast<uint4*>(tile + row * 128 + (lane & 7) * 16);
-      if (!sp.some(k + row, 1)) {
-        *at = make_uint4(0u, 0u, 0u, 0u);
-        continue;
-      }
-      uint4 x = *at;
-      const uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                    __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-      if ((top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u) {
-        x.x &= ~not_finite(x.x);
-        x.y &= ~not_finite(x.y);
-        x.z &= ~not_finite(x.z);
-        x.w &= ~not_finite(x.w);
-        *at = x;
-        bad[w] |= 1u << (row & 31);
+      const int row = (i0 + i) * 4 + row0;
+      if (row >= end || (row < from && row >= head)) {   // no query sees it
+        *reinterpret_cast<uint4*>(mine + (i0 + i) * 512) = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        acc[0] = taint(x[i].x, acc[0]);
+        acc[1] = taint(x[i].y, acc[1]);
+        acc[2] = taint(x[i].z, acc[2]);
+        acc[3] = taint(x[i].w, acc[3]);
       }
     }
   }
+  __syncwarp();
+  const uint32_t found = not_finite(acc[0]) | not_finite(acc[1]) | not_finite(acc[2]) | not_finite(acc[3]);
+  if (__any_sync(0xffffffffu, found != 0u)) {
+    uint32_t bad[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) bad[w] = __reduce_or_sync(0xffffffffu, bad[w]);
-  if (lane == 0 && e < MAX_EDGE) {
-    sy->edge_key[e] = k;
+    for (int w = 0; w < 4; ++w) {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const int row = w * 32 + i * 4;
+        uint4* at = reinterpret_cast<uint4*>(mine + row * 128);
+        uint4 x = *at;
+        const uint4 nf = make_uint4(not_finite(x.x), not_finite(x.y), not_finite(x.z), not_finite(x.w));
+        if (nf.x | nf.y | nf.z | nf.w) {
+          *at = make_uint4(x.x & ~nf.x, x.y & ~nf.y, x.z & ~nf.z, x.w & ~nf.w);
+          bad[w] |= 1u << (i * 4 + (lane >> 3));
+        }
+      }
+    }
 #pragma unroll
-    for (int w = 0; w < 4; ++w) sy->edge_bad[e][w] = bad[w];
-    if (bad[0] | bad[1] | bad[2] | bad[3]) sy->edges = e + 1;   // a clean tile's entry is used again
+    for (int w = 0; w < 4; ++w) bad[w] = __reduce_or_sync(0xffffffffu, bad[w]);
+    if (lane == 0 && e < MAX_EDGE) {
+      sy->edge_key[e] = k;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sy->edge_bad[e][w] = bad[w];
+      sy->edges = e + 1;
+    }
   }
   fence_proxy_async();
   __syncwarp();
 }
 
-__device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-          taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+// 8 consecutive fp32 columns of this thread's TMEM lane, waited for.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+  tmem_ld_wait();
 }
 
-// P = 2^(scale2 v - mu) of a row's tile in bf16 into tensor memory; returns its
-// sum.  A quarter of the exponentials run as a polynomial, which never gives
-// an exact 0, so a tile with masked keys (-inf) takes none.
-template <bool EDGE>
-__device__ __forceinline__ float weights(const float (&v)[BN], float scale2, float mu, uint32_t col) {
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+// P = 2^(scale2 v - mu) of 32 of a row's keys in bf16 into tensor memory;
+// returns their sum.
+__device__ __forceinline__ float weights(const float (&v)[32], float scale2, float mu, uint32_t col) {
+  const uint64_t sc = pair(scale2, scale2), base = pair(-mu, -mu);
+  uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-  for (int c = 0; c < BN; c += 32) {
-    uint32_t w[16];
+  for (int c = 0; c < 32; c += 16) {
+    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float x = fast_exp2(fmaf(v[c + i], scale2, -mu));
-      const float a = fmaf(v[c + i + 1], scale2, -mu);
-      const float y = !EDGE && (i & 2) ? poly_exp2(a) : fast_exp2(a);
-      sum[i & 2] += x;
-      sum[(i & 2) + 1] += y;
-      const __nv_bfloat162 xy = __floats2bfloat162_rn(x, y);
-      w[i / 2] = *reinterpret_cast<const uint32_t*>(&xy);
+    for (int i = 0; i < 8; ++i) {
+      float e0, e1;
+      split(fma2(pair(v[c + 2 * i], v[c + 2 * i + 1]), sc, base), e0, e1);
+      e0 = fast_exp2(e0);
+      e1 = fast_exp2(e1);
+      sum[i & 1] = add2(sum[i & 1], pair(e0, e1));
+      const __nv_bfloat162 xy = __floats2bfloat162_rn(e0, e1);
+      w[i] = *reinterpret_cast<const uint32_t*>(&xy);
     }
-    tmem_st16_async(col + c / 2, w);
+    tmem_st8_async(col + c / 2, w);
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  float a, b;
+  split(add2(sum[0], sum[1]), a, b);
+  return a + b;
 }
 
-constexpr int SMEM = 1024 + TILE + SLOTS * TILE + static_cast<int>(sizeof(Sync));
-// At most two CTAs fit on an SM (2 x 256 TMEM columns = all 512): tcgen05.alloc never waits.
-static_assert(2 * (SMEM + 1024) <= 228 * 1024 && 3 * (SMEM + 1024) > 228 * 1024, "two CTAs per SM");
+// The two warps of a query tile's row quarter (named barriers 1 to 8).
+__device__ __forceinline__ void quarter_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id + 1) : "memory"); }
+// Turns at the exponentials (named barriers 9 and 10): query tile x waits for
+// its turn, and gives the other its.
+__device__ __forceinline__ void turn_wait(int x) {
+  asm volatile("bar.sync %0, %1;" ::"r"(9 + x), "n"(2 * SM_WARPS * 32) : "memory");
+}
+__device__ __forceinline__ void turn_give(int x) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(9 + x), "n"(2 * SM_WARPS * 32) : "memory");
+}
 
-__global__ void __launch_bounds__(THREADS, 2)
+constexpr int SMEM = 1024 + (TILES + KS + VS) * TILE + static_cast<int>(sizeof(Sync));
+// One CTA per SM (it holds all 512 TMEM columns): tcgen05.alloc never waits.
+static_assert(SMEM <= 227 * 1024 && 2 * SMEM > 228 * 1024, "one CTA per SM");
+
+template <int PAGE>
+__global__ void __launch_bounds__(THREADS, 1)
     attend_kernel(const Params p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   const int b = blockIdx.z, g = blockIdx.y;
   int qbeg, nq, ntok, list0;
   if (!entry_ok(p, b, qbeg, nq, ntok, list0)) return;
   // the longest rows first: the last queries see the most keys
-  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * QT;
+  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * (TILES * QT);
   if (q0 >= nq) return;
   const int prefix = ntok - nq;
-  const Span sp(p, prefix + q0, prefix + min(nq, q0 + QT) - 1);
+  const int groups = nq - q0 > QT ? 2 : 1;   // query tiles with a query
+  const Span sp(p, prefix + q0, prefix + min(nq, q0 + TILES * QT) - 1);
   const int ntiles = sp.ntiles;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
   const uint32_t qtile = smem_addr(sm);
-  const uint32_t ring = qtile + TILE;
-  Sync* sy = reinterpret_cast<Sync*>(sm + TILE + SLOTS * TILE);
+  uint8_t *kring = sm + TILES * TILE, *vring = kring + KS * TILE;
+  Sync* sy = reinterpret_cast<Sync*>(vring + VS * TILE);
   volatile int* abort = &sy->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&sy->full[s], 1);
-      mbar_init(&sy->empty[s], 1);
+    for (int i = 0; i < KS; ++i) {
+      mbar_init(&sy->kfull[i], 1);
+      mbar_init(&sy->kempty[i], 1);
     }
-    mbar_init(&sy->sfull, 1);
-    mbar_init(&sy->sempty, SM_WARPS);
-    mbar_init(&sy->pfull, SM_WARPS);
-    mbar_init(&sy->pempty, 1);
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(&sy->vfull[i], 1);
+      mbar_init(&sy->vempty[i], 1);
+    }
+    for (int i = 0; i < TILES; ++i) {
+      mbar_init(&sy->sfull[i], 1);
+      mbar_init(&sy->sempty[i], SM_WARPS);
+      mbar_init(&sy->pfull[i], SM_WARPS);
+      mbar_init(&sy->pempty[i], 1);
+    }
     mbar_init(&sy->once, 1);
-    mbar_init(&sy->odone, 2);   // the last product and the MMA thread (its notes are in place)
-    mbar_init(&sy->mma_done, 1);
+    mbar_init(&sy->odone, 2);   // the last product and the PV thread (its notes are in place)
+    mbar_init(&sy->s_done, 1);
+    mbar_init(&sy->pv_done, 1);
     sy->abort = 0;
     sy->edges = 0;
     fence_mbar_init();
   }
-  if (warp == MMA_WARP) tmem_alloc(&sy->tmem, TMEM_COLS);
+  if (warp == S_WARP) tmem_alloc(&sy->tmem, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sy->tmem;
 
-  // Ring order: K(0), then for t = 1 ..: K(t), V(t - 1); V(ntiles - 1) last.
-  // Position i of it is K(0) for i = 0, K((i + 1) / 2) for odd i < 2 ntiles - 1
-  // and V(i / 2 - 1) for even i > 0; the last one, 2 ntiles - 1, is V(ntiles - 1).
-  if (warp == LOAD_WARP) {
-    const int total = 2 * ntiles;
-    const bool tma = p.P >= 8;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&sy->once, TILE);
-      tma_load_3d(sm, &qmap, 0, g * GROUP, qbeg + q0, &sy->once);
-    }
-    int i = 0;
-    for (; i < total; ++i) {
-      const int s = i % SLOTS;
-      const bool is_v = i > 0 && ((i & 1) == 0 || i == total - 1);
-      const int t = i == 0 ? 0 : i == total - 1 ? ntiles - 1 : is_v ? i / 2 - 1 : (i + 1) / 2;
-      if (i >= SLOTS && !warp_wait(&sy->empty[s], ((i / SLOTS) & 1) ^ 1, p.err, abort, lane)) {
-        *abort = 1;
-        break;
+  if (warp >= K_WARP) {
+    if (warp == K_WARP) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sy->once, groups * TILE);
+        for (int x = 0; x < groups; ++x)
+          tma_load_3d(sm + x * TILE, &qmap, 0, g * GROUP, qbeg + q0 + x * QT, &sy->once);
       }
-      if (tma) {
-        tma_tile(p, sp, is_v ? &vmap : &kmap, sm + TILE + s * TILE, &sy->full[s], list0, sp.key(t), g, lane);
-        continue;
-      }
-      copy_tile(p, sp, is_v ? p.v : p.k, ring + s * TILE, list0, sp.key(t), g, lane);
-      cp_async_commit();
-      if (i >= LAG) {
-        cp_async_wait<LAG>();
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sy->full[(i - LAG) % SLOTS]);
-      }
-    }
-    if (!tma) {
-      cp_async_wait<0>();
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0 && !*abort)
-        for (int u = max(0, i - LAG); u < i; ++u) mbar_arrive(&sy->full[u % SLOTS]);
-    }
-    if (lane == 0) {   // every issued load lands before the CTA may exit
-      if (tma)
-        for (int u = max(0, i - SLOTS); u < i; ++u) mbar_wait(&sy->full[u % SLOTS], (u / SLOTS) & 1, p.err);
-      mbar_wait(&sy->once, 0, p.err);
-    }
-  } else if (warp == MMA_WARP) {
-    bool issued = false, ok = warp_wait(&sy->once, 0, p.err, abort, lane);
-    int i = 0;   // ring position
-    for (int t = 0; t <= ntiles && ok; ++t) {
-      if (t < ntiles) {
-        const int s = i % SLOTS;
-        ok = warp_wait(&sy->full[s], (i / SLOTS) & 1, p.err, abort, lane) &&
-             (t == 0 || warp_wait(&sy->sempty, (t - 1) & 1, p.err, abort, lane));
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint64_t qdesc = sw128_desc(qtile), kdesc = sw128_desc(ring + s * TILE);
+      load_tiles<PAGE, KS>(p, sp, &kmap, p.k, kring, sy->kfull, sy->kempty, list0, g, lane, abort);
+      if (lane == 0) mbar_wait(&sy->once, 0, p.err);
+    } else if (warp == V_WARP) {
+      load_tiles<PAGE, VS>(p, sp, &vmap, p.v, vring, sy->vfull, sy->vempty, list0, g, lane, abort);
+    } else if (warp == S_WARP) {
+      const uint64_t qdesc = sw128_desc(qtile), kdesc = sw128_desc(smem_addr(kring));
+      bool ok = warp_wait_quiet(&sy->once, 0, p.err, abort, lane);
+      int t = 0;
+      for (; t < ntiles && ok; ++t) {
+        const int s = t % KS;
+        ok = warp_wait_quiet(&sy->kfull[s], (t / KS) & 1, p.err, abort, lane);
+        const uint64_t kd = kdesc + static_cast<uint64_t>(s * (TILE >> 4));
+        for (int x = 0; x < groups && ok; ++x) {
+          ok = t == 0 || warp_wait_quiet(&sy->sempty[x], (t - 1) & 1, p.err, abort, lane);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint64_t qd = qdesc + static_cast<uint64_t>(x * (TILE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) tc_mma(tmem, qdesc + 2 * kk, kdesc + 2 * kk, IDESC_S, kk > 0);
-          tc_commit(&sy->sfull);
-          tc_commit(&sy->empty[s]);
+            for (int kk = 0; kk < D / 16; ++kk) tc_mma(tmem + x * TMEM_TILE, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk > 0);
+            tc_commit(&sy->sfull[x]);
+            if (x + 1 == groups) tc_commit(&sy->kempty[s]);
+          }
         }
-        issued = true;
-        ++i;
       }
-      if (t >= 1) {
-        const int u = t - 1, s = i % SLOTS;
-        ok = warp_wait(&sy->full[s], (i / SLOTS) & 1, p.err, abort, lane);
+      if (lane == 0) {
+        if (!ok) *abort = 1;
+        tc_commit(&sy->s_done);   // every product completes before the tensor memory may be freed
+        mbar_wait(&sy->s_done, 0, p.err);
+      }
+    } else {
+      const uint64_t vdesc = sw128_mn_desc(smem_addr(vring));
+      bool ok = true;
+      for (int t = 0; t < ntiles && ok; ++t) {
+        const int s = t % VS;
+        ok = warp_wait_quiet(&sy->vfull[s], (t / VS) & 1, p.err, abort, lane);
         if (!ok) break;
-        if (!sp.whole(sp.key(u))) clean_values(sp, sm + TILE + s * TILE, sp.key(u), sy, lane);
-        ok = warp_wait(&sy->pfull, u & 1, p.err, abort, lane);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t vt = ring + s * TILE;
+        if (!sp.whole(sp.key(t))) clean_values(sp, vring + s * TILE, sp.key(t), sy, lane);
+        const uint64_t vd = vdesc + static_cast<uint64_t>(s * (TILE >> 4));
+        for (int x = 0; x < groups && ok; ++x) {
+          ok = warp_wait_quiet(&sy->pfull[x], t & 1, p.err, abort, lane);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t base = tmem + x * TMEM_TILE;
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            tc_mma_ts(tmem + O_COL, tmem + P_COL + kk * 8, sw128_mn_desc(vt + kk * 2048), IDESC_PV, u > 0 || kk > 0);
-          tc_commit(&sy->pempty);
-          tc_commit(&sy->empty[s]);
+            for (int kk = 0; kk < BN / 16; ++kk)
+              tc_mma_ts(base + O_COL, base + P_COL + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, t > 0 || kk > 0);
+            tc_commit(&sy->pempty[x]);
+            if (x + 1 == groups) tc_commit(&sy->vempty[s]);
+          }
         }
-        ++i;
       }
-    }
-    if (lane == 0) {
-      if (ok) {
-        mbar_arrive(&sy->odone);
-        tc_commit(&sy->odone);
-      } else {
-        *abort = 1;
-      }
-      if (issued) {   // every MMA completes before the tensor memory may be freed
-        tc_commit(&sy->mma_done);
-        mbar_wait(&sy->mma_done, 0, p.err);
+      if (lane == 0) {
+        if (ok) {
+          mbar_arrive(&sy->odone);
+          tc_commit(&sy->odone);
+        } else {
+          *abort = 1;
+        }
+        tc_commit(&sy->pv_done);
+        mbar_wait(&sy->pv_done, 0, p.err);
       }
     }
     __syncwarp();
-  } else {
-    const int r = warp * 32 + lane;              // accumulator row = TMEM lane
-    const int q = q0 + r / GROUP;
+  } else if (warp / SM_WARPS < groups) {
+    const int tile = warp / SM_WARPS, quarter = warp & 3, half = (warp >> 2) & 1;
+    const int r = quarter * 32 + lane;           // accumulator row = TMEM lane
+    const int q = q0 + tile * QT + r / GROUP;
     const int h = g * GROUP + r % GROUP;
     const int pos = prefix + min(q, nq - 1);
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t lanes = tmem + tile * TMEM_TILE + (static_cast<uint32_t>(quarter * 32) << 16);
+    // the positions of this warp's rows: a key tile that all of them see in
+    // full needs no mask, whatever the CTA's other rows see
+    Span own = sp;
+    own.p_lo = prefix + min(q0 + tile * QT + quarter * 4, nq - 1);
+    own.p_hi = prefix + min(q0 + tile * QT + quarter * 4 + 3, nq - 1);
+    float (&top)[2][2][BM] = sy->top[tile];
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    if (groups == 2 && tile == 1) turn_give(0);   // tile 0 begins
+    bool ok = true;   // after a timeout a warp only keeps its partner's barriers
     for (int t = 0; t < ntiles; ++t) {
-      if (!warp_wait(&sy->sfull, t & 1, p.err, abort, lane)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float v[BN];
-      __syncwarp();
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) tmem_ld32_async(lanes + c, v + c);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sy->sempty);   // the values are in registers
+      ok = ok && warp_wait_quiet(&sy->sfull[tile], t & 1, p.err, abort, lane);
+      float mt = -INFINITY;
       const int k0 = sp.key(t);
-      const bool edge = !sp.whole(k0);
-      if (edge) {
-        const int hi = pos - k0, lo = sp.window < 0 || hi < 0 ? -1 : hi - sp.window, fi = sp.first - k0;
+      const bool edge = !own.whole(k0);
+      const uint32_t scol = lanes + half * HALF;
+      // keys of this thread's half that its row sees: i <= hi and (i > lo or i < fi)
+      const int hi = pos - k0 - half * HALF, fi = sp.first - k0 - half * HALF;
+      const int lo = sp.window < 0 || hi < 0 ? -1 : hi - sp.window;
+      // The logits are read twice, 32 at a time, rather than kept: 64 of them do
+      // not fit beside the rest in the 96 registers of a thread among 640.
+      auto logits = [&](int c, float (&v)[32]) {
+        __syncwarp();
+        tmem_ld32(scol + c, v);
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < BN; ++i) v[i] = (i <= hi && (i > lo || i < fi)) ? v[i] : -INFINITY;
+          for (int i = 0; i < 32; ++i) v[i] = (c + i <= hi && (c + i > lo || c + i < fi)) ? v[i] : -INFINITY;
+        }
+      };
+      if (ok) {
+        tc_fence_after();
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < HALF; c += 32) {
+          float v[32];
+          logits(c, v);
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[i + 2 * k], v[i + 2 * k + 1]);
+        }
+        mt = p.scale2 * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        top[t & 1][half][r] = mt;
       }
-      float mx[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx[i] = v[i];
-#pragma unroll
-      for (int i = 8; i < BN; ++i) mx[i & 7] = fmaxf(mx[i & 7], v[i]);
-      const float mt = p.scale2 * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                        fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-      if (t >= 1 && !warp_wait(&sy->pempty, (t - 1) & 1, p.err, abort, lane)) {
-        ok = false;
-        break;
+      quarter_sync(tile * 4 + quarter);
+      ok = ok && (t == 0 || warp_wait_quiet(&sy->pempty[tile], (t - 1) & 1, p.err, abort, lane));
+      if (groups == 2) turn_wait(tile);
+      if (!ok) {
+        if (groups == 2 && (tile == 0 || t + 1 < ntiles)) turn_give(tile ^ 1);
+        continue;
       }
+      mt = fmaxf(mt, top[t & 1][half ^ 1][r]);
       tc_fence_after();
       const bool grow = mt > m + LAZY || (m == -INFINITY && mt > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
@@ -436,36 +522,47 @@ __global__ void __launch_bounds__(THREADS, 2)
         const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
         l *= a;
         m = mn;
-        if (t >= 1) {   // P V(t - 1) has completed: O is at rest
-          float o[32];
+        if (t >= 1) {   // P V(t - 1) has completed: O is at rest; each half takes 32 of its columns
           __syncwarp();
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            tmem_ld32(lanes + O_COL + c, o);
-            uint32_t w[32];
+          for (int c = 0; c < 32; c += 8) {   // a few columns at a time: the tile's logits stay in registers
+            float o[8];
+            tmem_ld8(lanes + O_COL + half * 32 + c, o);
+            uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * a);
-            tmem_st16_async(lanes + O_COL + c, w);
-            tmem_st16_async(lanes + O_COL + c + 16, w + 16);
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(o[i] * a);
+            tmem_st8_async(lanes + O_COL + half * 32 + c, w);
           }
         }
       }
       const float mu = m == -INFINITY ? 0.f : m;
-      __syncwarp();
-      l += edge ? weights<true>(v, p.scale2, mu, lanes + P_COL) : weights<false>(v, p.scale2, mu, lanes + P_COL);
+      const uint32_t pcol = lanes + P_COL + half * (HALF / 2);
+#pragma unroll
+      for (int c = 0; c < HALF; c += 32) {
+        float v[32];
+        logits(c, v);
+        if (c + 32 == HALF) {   // S is read: the next product may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sy->sempty[tile]);
+        }
+        l += weights(v, p.scale2, mu, pcol + c / 2);
+      }
+      if (groups == 2 && (tile == 0 || t + 1 < ntiles)) turn_give(tile ^ 1);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sy->pfull);
+      if (lane == 0) mbar_arrive(&sy->pfull[tile]);
     }
     if (!ok) *abort = 1;
-    if (ok && warp_wait(&sy->odone, 0, p.err, abort, lane)) {
+    top[ntiles & 1][half][r] = l;
+    quarter_sync(tile * 4 + quarter);
+    if (ok && warp_wait_quiet(&sy->odone, 0, p.err, abort, lane)) {
+      l += top[ntiles & 1][half ^ 1][r];
       tc_fence_after();
-      float o[D];
+      float o[32];
       __syncwarp();
-      tmem_ld32_async(lanes + O_COL, o);
-      tmem_ld32_async(lanes + O_COL + 32, o + 32);
-      tmem_ld_wait();
+      tmem_ld32(lanes + O_COL + half * 32, o);
       if (p.sinks) l += exp2f(p.sinks[h] * LOG2E - m);
       float f = 1.f / l;
       for (int e = 0; e < min(sy->edges, MAX_EDGE); ++e)
@@ -474,9 +571,9 @@ __global__ void __launch_bounds__(THREADS, 2)
             if (sp.sees(pos, sy->edge_key[e] + w * 32 + __ffs(bad) - 1)) f = __int_as_float(0x7fc00000);
       if (q < nq) {
         uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(qbeg + q) * p.o_st +
-                                              static_cast<int64_t>(h) * p.o_sh);
+                                              static_cast<int64_t>(h) * p.o_sh + half * 32);
 #pragma unroll
-        for (int c = 0; c < D; c += 8) {
+        for (int c = 0; c < 32; c += 8) {
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -491,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
+  if (warp == S_WARP) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 }  // namespace window
@@ -569,9 +666,12 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   p.o_st = o_st;
   p.o_sh = o_sh;
   p.err = err;
-  if (!host::set_smem(attend_kernel, SMEM)) return host::fail(CE_ERR_CUDA, "ce_window_prefill: smem attr");
-  const dim3 grid((max_q + QT - 1) / QT, num_kv_heads, bs);
-  attend_kernel<<<grid, THREADS, SMEM, static_cast<cudaStream_t>(stream)>>>(p, qmap, kmap, vmap);
+  if (!host::set_smem(attend_kernel<16>, SMEM) || !host::set_smem(attend_kernel<0>, SMEM))
+    return host::fail(CE_ERR_CUDA, "ce_window_prefill: smem attr");
+  const dim3 grid((max_q + TILES * QT - 1) / (TILES * QT), num_kv_heads, bs);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (page_size == 16) attend_kernel<16><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
+  else attend_kernel<0><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
   if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_window_prefill launch");
   return CE_OK;
 }

@@ -6,8 +6,7 @@ bf16 products, off by at most d = 80 * 2^-24 * scale * sum |q k|; a p is off by
 at most the relative e = 2 d + 16 * 2^-24 * (1 + |logit range|).  The decode form
 splits p into two bf16 parts (2^-17), so |error| <= (2^-17 + e) sum p |v| plus the
 output's rounding (2^-8 in bf16, 2^-24 in fp32).  The prefill form rounds p to
-bf16 (2^-8 of each) and takes a share of its exponentials from a polynomial
-(2^-13, coefficients' fit 7.6e-5): |error| <= (2^-8 + 2^-12 + e) sum p |v| + 2^-8 |o|.
+bf16 (2^-8 of each): |error| <= (2^-8 + e) sum p |v| + 2^-8 |o|.
 """
 import math
 
@@ -70,7 +69,7 @@ def hold(got, q, k, v, seen, sink, bf16_p, lse=None, f32=False):
     span = torch.where(seen[:, None], (z - l[..., None]).abs(), 0.0).amax(-1)
     e = 2 * d + 16 * 2.0 ** -24 * (1 + span)
     e = torch.where(l.isinf(), 0.0, e)[..., None]
-    w = 2.0 ** -8 + 2.0 ** -12 if bf16_p else 2.0 ** -17
+    w = 2.0 ** -8 if bf16_p else 2.0 ** -17
     tol = (w + e) * torch.einsum("njt,td->njd", p, v.abs()) + (2.0 ** -24 if f32 else 2.0 ** -8) * o.abs() + 1e-30
     bad = ((got.double() - o).abs() / tol)
     assert not got.isnan().any() and (bad <= 1).all(), float(bad.nan_to_num(1e9).max())
