@@ -19,6 +19,11 @@ eviction state (tables, positions, scores, pools) lives on the device.  With
 tensor parallelism each rank holds kv_heads/tp heads of every row; the only
 cross-rank exchange on the eviction path is the all-gather of per-head scores
 that H2O global needs at a boundary (tp.py adds the attention-output reduction).
+
+With kv_bits=4 the pools hold 4-bit pages (576 instead of 2,048 bytes per page
+and head): write_layer quantises the new tokens into them, decode_layer attends
+to them and run_boundaries moves them as they are.  Rows, tables, scores and
+policies are the same.
 """
 from __future__ import annotations
 
@@ -50,7 +55,12 @@ class RaggedDecodeEngine:
                  pool_units: int, max_rows: int, r2u_width: int, pos_cap: int,
                  device="cuda", head_offset: int = 0, global_kv_heads: Optional[int] = None,
                  process_group=None, alloc_pools: bool = True, boundary_rows: int = 8,
-                 hazard_bytes: int = 512 << 20, overlap_scores: bool = False):
+                 hazard_bytes: int = 512 << 20, overlap_scores: bool = False, kv_bits: int = 16):
+        if kv_bits not in (16, 4):
+            raise ValueError(f"kv_bits must be 16 or 4, not {kv_bits}")
+        if kv_bits == 4 and page_size != 16:
+            raise ValueError(f"4-bit pages hold 16 tokens, not {page_size}")
+        self.kv_bits = kv_bits
         self.L, self.H, self.G, self.P = layers, q_heads, kv_heads, page_size
         self.units = pool_units
         self.device = torch.device(device)
@@ -59,9 +69,12 @@ class RaggedDecodeEngine:
         self.group = process_group
         dev = self.device
         if alloc_pools:
-            shape = (pool_units, kv_heads, page_size, D)
-            self.k = [torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(layers)]
-            self.v = [torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(layers)]
+            def pool():
+                if kv_bits == 4:
+                    return kernels.kv4_pool(pool_units, kv_heads, dev)
+                return torch.empty((pool_units, kv_heads, page_size, D), dtype=torch.bfloat16, device=dev)
+            self.k = [pool() for _ in range(layers)]
+            self.v = [pool() for _ in range(layers)]
             self.kptr = kernels.layer_pointers(self.k, dev)
             self.vptr = kernels.layer_pointers(self.v, dev)
         self.scores = torch.zeros((layers, kv_heads, pool_units), dtype=torch.float32, device=dev)
@@ -120,7 +133,7 @@ class RaggedDecodeEngine:
             kernels.prepare_device(dev)
             kernels.reserve_boundary(dev, min(max_rows, boundary_rows), layers, kv_heads, page_size,
                                      r2u_width, pos_cap,
-                                     self.global_G if process_group is not None else 0, hazard_bytes)
+                                     self.global_G if process_group is not None else 0, hazard_bytes, kv_bits)
 
     def new_score_events(self):
         """Fresh ordering events for the score stream.  Also for a CUDA-graph
@@ -331,7 +344,7 @@ class RaggedDecodeEngine:
             self.vptr, self.G, P, rows_t, params_t, max_cols, max_n, live, marks=self.marks,
             epoch=self.epoch, swa=swa, uniforms=uniforms, global_scores=gscores,
             head_offset=self.head_offset, hazard_bytes=hazard_bytes, err=self.err,
-            max_width=max(prm["budget"] for prm in params))
+            max_width=max(prm["budget"] for prm in params), kv_bits=self.kv_bits)
         end.record()
         res = result.cpu().numpy()   # one readback per boundary batch, as the reference syncs
         self.boundary_ms.append(start.elapsed_time(end))
@@ -374,13 +387,43 @@ class RaggedDecodeEngine:
         depends on a buffer that another engine may regrow."""
         key = (bs, self.kv_indices.numel(), score_flags)
         if self._ws_need[0] != key:      # the same for every layer of a step
-            self._ws_need = (key, kernels.decode_workspace_bytes(bs, key[1], self.H, self.G, self.P,
-                                                                 score_flags))
+            if self.kv_bits == 4:
+                need = kernels.kv4_decode_workspace_bytes(bs, key[1], self.H, self.G, score_flags)
+            else:
+                need = kernels.decode_workspace_bytes(bs, key[1], self.H, self.G, self.P, score_flags)
+            self._ws_need = (key, need)
         need = self._ws_need[1]
         if self._dec_ws[k] is None or self._dec_ws[k].numel() < need:
             self.join_scores()
             self._dec_ws[k] = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self._dec_ws[k]
+
+    def _decode(self, layer, q, out, sinks, scale, score_flags, ws):
+        bs = len(self.active)
+        page = () if self.kv_bits == 4 else (self.P,)
+        decode = kernels.kv4_decode_attn_score if self.kv_bits == 4 else kernels.decode_attn_score
+        return decode(
+            q, self.k[layer], self.v[layer], self.kv_indptr[:bs + 1], self.kv_indices,
+            self.kv_tokens[:bs], scale, *page, sinks=sinks, mode_of_row=self.mode,
+            rows=self.rows_dev, scores=self.scores[layer], zero_new=True, out=out,
+            score_flags=score_flags, err=self.err, workspace=ws)
+
+    def slots(self) -> torch.Tensor:
+        """Slot (unit * page + position in the page) of every active row's
+        newest token, in batch order, after advance(): what write_layer takes,
+        the same for every layer.  Capturable."""
+        at = self.seq_lens_dev - 1
+        return self.r2u[self.rows_dev, at // self.P].long() * self.P + at % self.P
+
+    def write_layer(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
+        """K and V rows [rows, kv_heads, 64] bf16 of the active rows' newest
+        tokens into their slots of layer's pools, quantised with kv_bits=4."""
+        if self.kv_bits == 4:
+            kernels.kv4_write(k, v, self.k[layer], self.v[layer], slots, err=self.err)
+            return
+        unit, at = slots // self.P, slots % self.P
+        self.k[layer][unit, :, at] = k
+        self.v[layer][unit, :, at] = v
 
     def decode_layer(self, layer: int, q: torch.Tensor, out: torch.Tensor, sinks, scale: float,
                      score_flags: Optional[int] = None):
@@ -388,11 +431,7 @@ class RaggedDecodeEngine:
         score_flags = self.score_flags if score_flags is None else score_flags
         if not (self.overlap_scores and score_flags & 3 and bs):
             ws = self._decode_workspace(0, bs, score_flags) if bs else None
-            return kernels.decode_attn_score(
-                q, self.k[layer], self.v[layer], self.kv_indptr[:bs + 1], self.kv_indices,
-                self.kv_tokens[:bs], scale, self.P, sinks=sinks, mode_of_row=self.mode,
-                rows=self.rows_dev, scores=self.scores[layer], zero_new=True, out=out,
-                score_flags=score_flags, err=self.err, workspace=ws)
+            return self._decode(layer, q, out, sinks, scale, score_flags, ws)
         # Attention and outputs on the current stream; this layer's page scores
         # on the score stream once they are done, overlapping the next layer.
         # Workspace k is reused two layers later, after its scores have run.
@@ -400,11 +439,7 @@ class RaggedDecodeEngine:
         ws = self._decode_workspace(k, bs, score_flags)
         main = torch.cuda.current_stream(self.device)
         main.wait_event(self._ws_free[k])
-        res = kernels.decode_attn_score(
-            q, self.k[layer], self.v[layer], self.kv_indptr[:bs + 1], self.kv_indices,
-            self.kv_tokens[:bs], scale, self.P, sinks=sinks, mode_of_row=self.mode,
-            rows=self.rows_dev, scores=self.scores[layer], zero_new=True, out=out,
-            score_flags=score_flags | capi.CE_SCORE_DEFER, err=self.err, workspace=ws)
+        res = self._decode(layer, q, out, sinks, scale, score_flags | capi.CE_SCORE_DEFER, ws)
         self._attn_done[k].record(main)
         side = self._score_stream
         side.wait_event(self._attn_done[k])
@@ -568,6 +603,13 @@ def synth_state(engine: RaggedDecodeEngine, specs: list, seed: int, score_sigma:
         engine.scores[:, :, idx] = vals.exp_()
     if fill_pools:
         gen = torch.Generator(device=engine.device).manual_seed(seed + 11)
-        for t in engine.k + engine.v:
-            t.normal_(generator=gen)
+        if engine.kv_bits == 4:
+            for k, v in zip(engine.k, engine.v):
+                for a in range(0, engine.units, 8192):
+                    n = min(8192, engine.units - a) * engine.P
+                    x = torch.randn((2, n, G, D), generator=gen, device=engine.device).to(torch.bfloat16)
+                    kernels.kv4_write(x[0], x[1], k, v, a * engine.P + torch.arange(n, device=engine.device))
+        else:
+            for t in engine.k + engine.v:
+                t.normal_(generator=gen)
     engine.commit_rows()

@@ -593,8 +593,10 @@ def layer_pointers(tensors: Sequence[torch.Tensor], device) -> torch.Tensor:
 def boundary(table, req_to_unit, frontier, count, pos, scores, k_ptrs, v_ptrs, kv_heads, page_size,
              rows, params, max_cols, max_n, live, marks=None, epoch=0, swa=None, uniforms=None,
              global_scores=None, head_offset=0, freed=None, hazard_bytes=256 << 20, err=None,
-             max_width=0, record=None):
-    """One eviction boundary for a batch of rows (runtime:415-507).
+             max_width=0, record=None, kv_bits=16):
+    """One eviction boundary for a batch of rows (runtime:415-507); with
+    kv_bits 4 over pools from kv4_pool (ce_kv4_boundary), whose pages move as
+    they are.
 
     record: None, or (delta [R * L * G, >= max_cols] int32 device tensor,
     counts [R * L * G] int32) to receive the retention record
@@ -608,16 +610,13 @@ def boundary(table, req_to_unit, frontier, count, pos, scores, k_ptrs, v_ptrs, k
     result = torch.zeros((max(R, 1), 4), dtype=torch.int32, device=dev)
     if freed is None:
         freed = torch.full((max(R, 1), max(max_cols, 1)), -1, dtype=torch.int32, device=dev)
-    need = lib.ce_boundary_workspace_bytes(R, L, kv_heads, 64, page_size, max_cols, int(max_width),
-                                           global_scores.shape[2] if global_scores is not None else 0,
-                                           hazard_bytes)
-    if need < 0:
-        raise capi.CeError("ce_boundary_workspace_bytes failed")
+    need = _boundary_bytes(R, L, kv_heads, page_size, max_cols, int(max_width),
+                           global_scores.shape[2] if global_scores is not None else 0, hazard_bytes, kv_bits)
     ws = WORKSPACES.get(dev, "boundary", need)
     udt = capi.CE_DTYPE_NONE
     if uniforms is not None:
         udt = capi.CE_DTYPE_F64 if uniforms.dtype == torch.float64 else capi.CE_DTYPE_F32
-    st = lib.ce_boundary(
+    st = (lib.ce_kv4_boundary if kv_bits == 4 else lib.ce_boundary)(
         _p(table), table.stride(0), table.shape[1], _p(req_to_unit), req_to_unit.stride(0),
         req_to_unit.shape[1], _p(frontier), _p(count), _p(pos), pos.stride(0), pos.shape[3],
         _p(scores), scores.stride(0), scores.stride(1), scores.shape[2], _p(k_ptrs), _p(v_ptrs), L,
@@ -627,14 +626,15 @@ def boundary(table, req_to_unit, frontier, count, pos, scores, k_ptrs, v_ptrs, k
         int(max_width), int(max_n), _p(result), _p(freed), freed.stride(0), _p(ws), ws.numel(), int(hazard_bytes),
         _p(record[0]) if record else None, record[0].stride(0) if record else 0,
         _p(record[1]) if record else None, _p(err), _stream(dev))
-    capi.check(st, "ce_boundary")
+    capi.check(st, "ce_kv4_boundary" if kv_bits == 4 else "ce_boundary")
     if R:
         # bsel, bvalidate, bfinish; hsum (and unit_sum for long rows that own
         # most of the pool) without global scores; bzero when
         # live; a gather and a scatter per launch group (rows x layers fitting
         # the hazard scratch)
         width = max_width if 0 < max_width < max_cols else max_cols
-        row_layer = max(1, kv_heads * width * 2 * page_size * 128)
+        slice_bytes = capi.CE_KV4_SLICE_BYTES if kv_bits == 4 else page_size * 128
+        row_layer = max(1, kv_heads * width * 2 * slice_bytes)
         hz = max(int(hazard_bytes), row_layer)
         rows_per = min(R, max(1, hz // row_layer))
         group = min(L, max(1, hz // (rows_per * row_layer)))
@@ -652,13 +652,27 @@ def prepare_device(device):
         capi.check(capi.load().ce_prepare_device(), "ce_prepare_device")
 
 
-def reserve_boundary(device, rows, layers, kv_heads, page_size, max_cols, max_width, global_heads,
-                     hazard_bytes):
-    """Allocate the ce_boundary workspace for the given batch bounds ahead of use."""
-    need = capi.load().ce_boundary_workspace_bytes(rows, layers, kv_heads, 64, page_size, max_cols,
-                                                   max_width, global_heads, hazard_bytes)
+def _boundary_bytes(rows, layers, kv_heads, page_size, max_cols, max_width, global_heads, hazard_bytes, kv_bits):
+    lib = capi.load()
+    if kv_bits == 4:
+        name = "ce_kv4_boundary_workspace_bytes"
+        need = lib.ce_kv4_boundary_workspace_bytes(rows, layers, kv_heads, 64, page_size, max_cols, max_width,
+                                                   hazard_bytes)
+    elif kv_bits == 16:
+        name = "ce_boundary_workspace_bytes"
+        need = lib.ce_boundary_workspace_bytes(rows, layers, kv_heads, 64, page_size, max_cols, max_width,
+                                               global_heads, hazard_bytes)
+    else:
+        raise capi.CeError("kv_bits must be 16 or 4")
     if need < 0:
-        raise capi.CeError("ce_boundary_workspace_bytes failed")
+        raise capi.CeError(f"{name} failed")
+    return need
+
+
+def reserve_boundary(device, rows, layers, kv_heads, page_size, max_cols, max_width, global_heads,
+                     hazard_bytes, kv_bits=16):
+    """Allocate the boundary workspace for the given batch bounds ahead of use."""
+    need = _boundary_bytes(rows, layers, kv_heads, page_size, max_cols, max_width, global_heads, hazard_bytes, kv_bits)
     return WORKSPACES.get(torch.device(device), "boundary", need)
 
 

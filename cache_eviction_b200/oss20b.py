@@ -110,10 +110,10 @@ class OssDecoder:
 
     eviction: the policy of the full layers (None: a full cache); scored=False
     keeps the same boundaries with H2O scoring off (the full-cache decode rate
-    at the same resident KV)."""
+    at the same resident KV); kv_bits=4 holds the full layers' pages in 4 bits."""
 
     def __init__(self, weights: OssWeights, eviction: Optional[EvictionConfig], max_len: int,
-                 scored: bool = True, device="cuda", page_size: int = 16):
+                 scored: bool = True, device="cuda", page_size: int = 16, kv_bits: int = 16):
         cfg = weights.cfg
         self.w, self.cfg = weights, cfg
         dev = self.device = torch.device(device)
@@ -126,7 +126,7 @@ class OssDecoder:
         self.eng = RaggedDecodeEngine(layers=len(self.full), q_heads=cfg.q_heads, kv_heads=cfg.kv_heads,
                                       page_size=P, pool_units=units, max_rows=1,
                                       r2u_width=-(-max_len // P) + 8, pos_cap=max(64, units), device=dev,
-                                      boundary_rows=1)
+                                      boundary_rows=1, kv_bits=kv_bits)
         self.eng.seed_free_units(list(range(1, units)))
         self.eng.add_row(0, eviction, 0)
         if not scored:
@@ -193,8 +193,11 @@ class OssDecoder:
             k = qk[Hq:].view(1, G, hd)
             v = qkv[:, (Hq + G) * hd:].view(1, G, hd)
             if cfg.full_layer(l):
-                eng.k[fi][unit, :, slot] = k
-                eng.v[fi][unit, :, slot] = v
+                if eng.kv_bits == 4:
+                    eng.write_layer(fi, k, v, unit * eng.P + slot)
+                else:
+                    eng.k[fi][unit, :, slot] = k
+                    eng.v[fi][unit, :, slot] = v
                 eng.decode_layer(fi, q, self.attn, lw["sinks"], self.scale)
                 fi += 1
             else:
