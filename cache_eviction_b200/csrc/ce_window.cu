@@ -5,15 +5,19 @@
 //   out_i = softmax over {t <= p, t > p - window or t < first} (and the sink) of
 //           scale q_i . k_t,  times v_t,    p = kv_tokens - nq + i
 //
-// One CTA per (32 queries, KV head, entry), two tiles of 16 queries whose 8
-// heads are a tile's 128 accumulator rows and share every key and value tile.
-// It walks the 128-key tiles that hold a visible token of some row (the first
-// tokens' tiles, then the window's, which start at a page boundary), in one pass:
-//   load warps    K tiles through one ring of 16 KB slots, V tiles through
-//                 another (page loads by TMA, or cp.async gathers for pages
-//                 under 8 tokens), page indices read a tile ahead
+// An item is (32 queries, KV head, entry): two tiles of 16 queries whose 8 heads
+// are a tile's 128 accumulator rows and share every key and value tile.  One
+// CTA per SM takes every gridDim-th item, the last queries (which see the most
+// keys) first, and walks the 128-key tiles that hold a visible token of some
+// row (the first tokens' tiles, then the window's, which start at a page
+// boundary), in one pass:
+//   load warp     picks the items; queries through two slots of 32 KB, key and
+//                 value tiles each through a ring of 16 KB slots (page loads by
+//                 TMA, or cp.async gathers for pages under 8 tokens), page
+//                 indices read a tile ahead
 //   S warp        S(t) = Q K^T of both query tiles into tensor memory, each as
 //                 soon as its S(t-1) is read
+//   clean warp    value tiles that are seen in part made safe (below)
 //   PV warp       O += P(t) V(t) of each once its weights are in place
 //   softmax warps eight per query tile, two threads per row, 64 keys each: S from
 //                 tensor memory, running maximum (exchanged through shared
@@ -22,11 +26,20 @@
 //                 rescaled only when a row's maximum has grown by more than
 //                 2^8 since the last rescale (P stays below 2^8, its relative
 //                 precision and the fp32 sum's are the same).
-// The exponentials bound the kernel (one per row and key on a unit of 16 per
-// clock and SM: 1,024 clocks per tile, against 768 of the tensor cores), so the
-// two query tiles take turns at them: while one computes its weights the
-// other's waits, reads and maxima go on.  Left to themselves (two CTAs per SM)
-// the tiles fell into step, both at the exponentials and then both waiting.
+// The warps go from item to item by themselves, through a ring of item slots:
+// an item's loads, first products and clean-up run under the one before.  (A CTA
+// per item left the SM idle while it started and ended: 207 us instead of 123
+// for prompts of 4,093 and 3,069 tokens, 64 heads, window 128, where an item
+// has two key tiles.)
+// The exponentials bound long items (one per row and key on a unit of 16 per
+// clock and SM: 2,048 clocks per key tile and item, against 1,536 of the tensor
+// cores), so the two query tiles take turns at them: while one computes its
+// weights the other's waits, reads and maxima go on.  Left to themselves (two
+// CTAs per SM) the tiles fell into step, both at the exponentials and then both
+// waiting.  2,048 queries behind 26,624 tokens (2,048 first + 6,144 window), 64
+// heads: 540 us, 509 TFLOP/s, ~4,000 clocks per key tile and item; its 512
+// items are 3.5 rounds of 148.  Short items are bound by their chain of waits
+// (last product, normaliser, output, then the next item's first maximum).
 // (Taking a share of the exponentials as a polynomial on the FMA pipes was
 // slower at every share.)  P in bf16 is rounded by at most 2^-9 of itself, less
 // than the output's own rounding makes of it on average; maxima, sums and O
@@ -34,12 +47,14 @@
 //
 // What a row must not see must not reach it: a masked key's logit is replaced
 // before the maximum, and a masked value meets P = 0, which is no help if it
-// is infinite or NaN.  So in a tile that some row sees only in part the PV
+// is infinite or NaN.  So in a tile that some row sees only in part the clean
 // warp clears the values that no row sees (a page's unwritten slots, pages that
 // were not loaded) and any value that is not finite, noting its token; a row
 // that does see such a token gets NaN at the end.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "ce_common.cuh"
 #include "ce_host.h"
@@ -55,12 +70,14 @@ constexpr int BN = 128;                  // keys per tile
 constexpr int QT = BM / GROUP;           // 16 queries per tile
 constexpr int TILES = 2;                 // query tiles per CTA
 constexpr int TILE = 128 * 128;          // 128 rows x 128 B
-constexpr int KS = 5, VS = 5;            // ring slots of K and V tiles
+constexpr int KS = 4, VS = 4;            // ring slots of K and V tiles
+constexpr int QS = 2;                    // items whose queries are in shared memory
+constexpr int IS = 4;                    // items between the load warp and the last one to finish with one
 constexpr int LAG = 3;                   // cp.async tiles in flight before one is published
 constexpr int SM_WARPS = 8;              // softmax, per query tile: TMEM lanes 32 (w % 4) .. +31, keys 64 (w / 4) .. +63
 constexpr int HALF = BN / 2;             // keys of a softmax thread
-constexpr int K_WARP = TILES * SM_WARPS, V_WARP = K_WARP + 1, S_WARP = K_WARP + 2;   // and the PV warp
-constexpr int THREADS = 32 * (TILES * SM_WARPS + 4);
+constexpr int L_WARP = TILES * SM_WARPS, C_WARP = L_WARP + 1, S_WARP = L_WARP + 2;   // load, clean, S and the PV warp
+constexpr int THREADS = 32 * (TILES * SM_WARPS + 4);   // (one warp more would leave a thread 80 registers)
 constexpr uint32_t TMEM_TILE = 256, TMEM_COLS = TILES * TMEM_TILE, P_COL = 128, O_COL = 192;   // S | P | O of each tile
 constexpr uint32_t IDESC_S = f16_idesc(BM, BN);
 constexpr uint32_t IDESC_PV = f16_idesc(BM, D) | kIdescBMajorMN;
@@ -75,6 +92,8 @@ struct Params {
   const float* sinks;
   float scale2;           // sm_scale * log2(e)
   int G, P;
+  int64_t items;          // query tile pairs x KV heads x entries
+  int bs, xs;             // entries, query tile pairs of the longest one
   int total_q, max_q, max_tokens;
   int window, first;
   __nv_bfloat16* out;
@@ -82,19 +101,29 @@ struct Params {
   int32_t* err;
 };
 
-struct Sync {
-  uint64_t kfull[KS], kempty[KS], vfull[VS], vempty[VS];
-  uint64_t sfull[TILES], sempty[TILES], pfull[TILES], pempty[TILES];
-  uint64_t once, odone, s_done, pv_done;
-  uint32_t tmem;
-  int abort;
-  float top[TILES][2][2][BM];     // by query tile, key tile parity and half: the rows' maxima; at the end their sums
-  int edges;                      // tiles in whose values the PV warp found some that are not finite
+// One (32 queries, KV head, entry).
+struct Item {
+  int64_t number;                 // p.items: no more of them
+  int g, q0, nq, prefix, qbeg, list0;
+};
+struct ItemSlot : Item {
+  int edges;                      // tiles in whose values the clean warp found some that are not finite
   int edge_key[MAX_EDGE];         // their first token
-  uint32_t edge_bad[MAX_EDGE][4]; // their tokens with a value that is not finite
+  uint32_t edge_bad[MAX_EDGE][4]; // their tokens with such a value
 };
 
-// The keys a CTA's rows (positions p_lo .. p_hi) see, as 128-key tiles.
+struct Sync {
+  uint64_t kfull[KS], kempty[KS], vfull[VS], vclean[VS], vempty[VS], qfull[QS], qempty[QS], ifull[IS], iempty[IS];
+  uint64_t sfull[TILES], sempty[TILES], pfull[TILES], pempty[TILES], odone[TILES];
+  uint64_t s_done, pv_done;
+  uint32_t tmem;
+  int abort;
+  ItemSlot items[IS];
+  float top[TILES][2][2][BM];     // by query tile, key tile parity and half: the rows' maxima
+  float sum[TILES][2][BM];        // and at the end of an item their sums
+};
+
+// The keys an item's rows (positions p_lo .. p_hi) see, as 128-key tiles.
 struct Span {
   int p_lo, p_hi, lo, first, window;   // lo: first key in some row's window
   int head, start, ntiles;             // tiles 0 .. head-1 at 128 t, the rest from `start` on
@@ -123,25 +152,72 @@ struct Span {
   }
 };
 
-__device__ __forceinline__ bool entry_ok(const Params& p, int b, int& qbeg, int& nq, int& ntok, int& list0) {
-  qbeg = p.qo_indptr[b];
-  nq = p.qo_indptr[b + 1] - qbeg;
-  ntok = p.kv_tokens[b];
-  list0 = p.kv_indptr[b];
+// Item `number`, if its entry's ranges fit and it has a query.  The last
+// queries, which see the most keys, come first.
+__device__ __forceinline__ bool make_item(const Params& p, int64_t number, Item& it) {
+  if (number >= p.items) return false;
+  const int64_t per = static_cast<int64_t>(p.G) * p.bs;
+  const int x = p.xs - 1 - static_cast<int>(number / per), gb = static_cast<int>(number % per), b = gb / p.G;
+  it.number = number;
+  it.g = gb % p.G;
+  it.q0 = x * (TILES * QT);
+  it.qbeg = p.qo_indptr[b];
+  it.nq = p.qo_indptr[b + 1] - it.qbeg;
+  it.list0 = p.kv_indptr[b];
+  const int ntok = p.kv_tokens[b], pages = p.kv_indptr[b + 1] - it.list0;
+  it.prefix = ntok - it.nq;
   const int64_t units = (static_cast<int64_t>(ntok) + p.P - 1) / p.P;
-  const bool ok = qbeg >= 0 && nq >= 0 && qbeg + static_cast<int64_t>(nq) <= p.total_q && nq <= p.max_q &&
-                  ntok <= p.max_tokens && ntok >= nq && list0 >= 0 && list0 + units <= p.kv_capacity &&
-                  units <= p.kv_indptr[b + 1] - list0;
-  if (!ok && threadIdx.x == 0 && blockIdx.x == 0) flag_error(p.err, CE_EW_SHAPE);
-  return ok;
+  const bool ok = it.qbeg >= 0 && it.nq >= 0 && it.qbeg + static_cast<int64_t>(it.nq) <= p.total_q && it.nq <= p.max_q &&
+                  ntok <= p.max_tokens && ntok >= it.nq && it.list0 >= 0 && it.list0 + units <= p.kv_capacity &&
+                  units <= pages;
+  if (!ok && x == 0) flag_error(p.err, CE_EW_SHAPE);
+  return ok && it.q0 < it.nq;
+}
+__device__ __forceinline__ int groups_of(const Item& it) { return it.nq - it.q0 > QT ? 2 : 1; }   // query tiles with a query
+__device__ __forceinline__ Span span_of(const Params& p, const Item& it) {
+  return Span(p, it.prefix + it.q0, it.prefix + min(it.nq, it.q0 + TILES * QT) - 1);
 }
 
-// A load warp's tiles of one pool through its ring.  PAGE: tokens per page, or
-// 0 for any size that divides 64.
-template <int PAGE, int SLOTS>
-__device__ __forceinline__ void load_tiles(const Params& p, const Span& sp, const CUtensorMap* map,
-                                           const __nv_bfloat16* pool, uint8_t* ring, uint64_t* full, uint64_t* empty,
-                                           int list0, int g, int lane, volatile int* abort) {
+// A position in a ring of n slots and the parity of its round.  (A wait for the
+// parity before the first, 1, is over at once: the slots are empty.)
+struct Ring {
+  int slot = 0, n;
+  uint32_t phase = 0;
+  __device__ __forceinline__ explicit Ring(int slots) : n(slots) {}
+  __device__ __forceinline__ void next() {
+    if (++slot == n) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// The i-th item of this CTA from its slot.  False: no more, or a wait gave up.
+__device__ __forceinline__ bool next_item(const Params& p, Sync* sy, int i, Item& it, bool& ok, int lane) {
+  ok = ok && warp_wait_quiet(&sy->ifull[i % IS], (i / IS) & 1, p.err, &sy->abort, lane);
+  if (!ok) return false;
+  __syncwarp();
+  it = sy->items[i % IS];
+  return it.number < p.items;
+}
+// Its slot may be used again (as far as this warp is concerned).
+__device__ __forceinline__ void release_item(Sync* sy, int i, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&sy->iempty[i % IS]);
+}
+
+// Where the load warp puts the tiles.
+struct Rings {
+  uint8_t *ktile, *vtile;
+  uint64_t *kfull, *kempty, *vfull, *vempty;
+  Ring k, v;
+};
+
+// The key and value tiles of one item into their rings; false once a wait gave
+// up.  PAGE: tokens per page, or 0 for any size that divides 64.
+template <int PAGE>
+__device__ __forceinline__ bool load_tiles(const Params& p, const Span& sp, Rings& at, const CUtensorMap* kmap,
+                                           const CUtensorMap* vmap, int list0, int g, int lane, volatile int* abort) {
   const int P = PAGE ? PAGE : p.P;
   const bool tma = P >= 8;
   // Pages of at least 8 rows: lane i < 128 / P the tile's page i.  Smaller ones:
@@ -154,64 +230,80 @@ __device__ __forceinline__ void load_tiles(const Params& p, const Span& sp, cons
     if (sp.some(k, tma ? P : 1)) flag_error(p.err, CE_EW_INDEX);
     return -1;
   };
-  int t = 0;
+  auto empty = [&](uint64_t* bars, const Ring& r) { return warp_wait_quiet(&bars[r.slot], r.phase ^ 1, p.err, abort, lane); };
   if (tma) {
     const int pages = BN / P;
     int next = lane < pages ? unit_of(sp.key(0) + lane * P) : -1;
-    for (; t < sp.ntiles; ++t) {
-      const int s = t % SLOTS, k0 = sp.key(t) + lane * P;
+    for (int t = 0; t < sp.ntiles; ++t) {
+      const int k0 = sp.key(t) + lane * P;
       const int unit = lane < pages ? checked(next, k0) : -1;
       if (t + 1 < sp.ntiles) next = lane < pages ? unit_of(sp.key(t + 1) + lane * P) : -1;
-      const unsigned valid = __ballot_sync(0xffffffffu, unit >= 0);
-      if (t >= SLOTS && !warp_wait_quiet(&empty[s], ((t / SLOTS) & 1) ^ 1, p.err, abort, lane)) {
-        *abort = 1;
-        break;
-      }
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(valid) * P * 128);
+      const int bytes = __popc(__ballot_sync(0xffffffffu, unit >= 0)) * P * 128, row = (unit * p.G + g) * P;
+      if (!empty(at.kempty, at.k)) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&at.kfull[at.k.slot], bytes);
       __syncwarp();
-      if (unit >= 0) tma_load_2d(ring + s * TILE + lane * P * 128, map, 0, (unit * p.G + g) * P, &full[s]);
+      if (unit >= 0) tma_load_2d(at.ktile + at.k.slot * TILE + lane * P * 128, kmap, 0, row, &at.kfull[at.k.slot]);
+      at.k.next();
+      if (!empty(at.vempty, at.v)) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&at.vfull[at.v.slot], bytes);
+      __syncwarp();
+      if (unit >= 0) tma_load_2d(at.vtile + at.v.slot * TILE + lane * P * 128, vmap, 0, row, &at.vfull[at.v.slot]);
+      at.v.next();
     }
-    if (lane == 0)   // every issued load lands before the CTA may exit
-      for (int u = max(0, t - SLOTS); u < t; ++u) mbar_wait(&full[u % SLOTS], (u / SLOTS) & 1, p.err);
-    return;
+    return true;
   }
   if constexpr (PAGE == 0) {
-    for (; t < sp.ntiles; ++t) {
-      const int s = t % SLOTS, k0 = sp.key(t);
-      int u[4];
-  #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = unit_of(k0 + lane + 32 * i);
-  #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = checked(u[i], k0 + lane + 32 * i);
-      if (t >= SLOTS && !warp_wait_quiet(&empty[s], ((t / SLOTS) & 1) ^ 1, p.err, abort, lane)) {
-        *abort = 1;
-        break;
+    auto publish = [&](int back) {   // the tile so many before the last
+      if (lane == 0) {
+        mbar_arrive(&at.kfull[(at.k.slot + KS - 1 - back) % KS]);
+        mbar_arrive(&at.vfull[(at.v.slot + VS - 1 - back) % VS]);
       }
+    };
+    bool ok = true;
+    int t = 0;
+    for (; t < sp.ntiles; ++t) {
+      const int k0 = sp.key(t);
+      int u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = unit_of(k0 + lane + 32 * i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = checked(u[i], k0 + lane + 32 * i);
+      ok = empty(at.kempty, at.k) && empty(at.vempty, at.v);
+      if (!ok) break;
+      const uint32_t kto = smem_addr(at.ktile) + at.k.slot * TILE, vto = smem_addr(at.vtile) + at.v.slot * TILE;
       const int c = lane & 7;
-  #pragma unroll 4
+#pragma unroll 4
       for (int j = 0; j < BN / 4; ++j) {
         const int r = (lane >> 3) + 4 * j;
         const int from = (j >> 3) == 0 ? u[0] : (j >> 3) == 1 ? u[1] : (j >> 3) == 2 ? u[2] : u[3];
         const int unit = __shfl_sync(0xffffffffu, from, r & 31);
-        const bool ok = unit >= 0;   // rows that no query sees are zeros
-        const __nv_bfloat16* src =
-            ok ? pool + ((static_cast<int64_t>(unit) * p.G + g) * P + (k0 + r) % P) * D + c * 8 : pool;
-        cp_async16(smem_addr(ring) + s * TILE + swz(r, c), src, ok);
+        const bool have = unit >= 0;   // rows that no query sees are zeros
+        const int64_t off = have ? ((static_cast<int64_t>(unit) * p.G + g) * P + (k0 + r) % P) * D + c * 8 : 0;
+        cp_async16(kto + swz(r, c), p.k + off, have);
+        cp_async16(vto + swz(r, c), p.v + off, have);
       }
+      at.k.next();
+      at.v.next();
       cp_async_commit();
       if (t >= LAG) {
         cp_async_wait<LAG>();
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[(t - LAG) % SLOTS]);
+        publish(LAG);
       }
     }
-    cp_async_wait<0>();
+    cp_async_wait<0>();   // an item's tiles are all published before the next one's
     fence_proxy_async();
     __syncwarp();
-    if (lane == 0 && !*abort)
-      for (int u = max(0, t - LAG); u < t; ++u) mbar_arrive(&full[u % SLOTS]);
+    if (ok)
+      for (int back = min(t, LAG) - 1; back >= 0; --back) publish(back);
+    return ok;
   }
+  return true;
+}
+// Every TMA load issued lands before the CTA may exit: the last round of each slot.
+__device__ __forceinline__ void drain(uint64_t* full, Ring at, int32_t* err) {
+  for (int s = 0; s < at.n; ++s) mbar_wait(&full[s], at.phase ^ (s >= at.slot ? 1u : 0u), err);
 }
 
 // Halves of a bf16 pair that are not finite, as masks.
@@ -229,8 +321,8 @@ __device__ __forceinline__ uint32_t taint(uint32_t w, uint32_t acc) {
 // A partly visible value tile (keys from k on) made safe for P = 0, by one warp:
 // rows that no query sees are cleared, then values that are not finite, whose
 // tokens are noted.
-__device__ __forceinline__ void clean_values(const Span& sp, uint8_t* tile, int k, Sync* sy, int lane) {
-  const int e = sy->edges;
+__device__ __forceinline__ void clean_values(const Span& sp, uint8_t* tile, int k, ItemSlot* it, int lane) {
+  const int e = it->edges;
   __syncwarp();
   uint8_t* mine = tile + (lane >> 3) * 128 + (lane & 7) * 16;
   const int row0 = lane >> 3, end = sp.p_hi + 1 - k, from = sp.lo - k, head = sp.first - k;
@@ -274,10 +366,10 @@ __device__ __forceinline__ void clean_values(const Span& sp, uint8_t* tile, int 
 #pragma unroll
     for (int w = 0; w < 4; ++w) bad[w] = __reduce_or_sync(0xffffffffu, bad[w]);
     if (lane == 0 && e < MAX_EDGE) {
-      sy->edge_key[e] = k;
+      it->edge_key[e] = k;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sy->edge_bad[e][w] = bad[w];
-      sy->edges = e + 1;
+      for (int w = 0; w < 4; ++w) it->edge_bad[e][w] = bad[w];
+      it->edges = e + 1;
     }
   }
   fence_proxy_async();
@@ -330,7 +422,10 @@ __device__ __forceinline__ void turn_give(int x) {
   asm volatile("bar.arrive %0, %1;" ::"r"(9 + x), "n"(2 * SM_WARPS * 32) : "memory");
 }
 
-constexpr int SMEM = 1024 + (TILES + KS + VS) * TILE + static_cast<int>(sizeof(Sync));
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); }
+
+constexpr int SMEM = 1024 + (QS * TILES + KS + VS) * TILE + static_cast<int>(sizeof(Sync));
 // One CTA per SM (it holds all 512 TMEM columns): tcgen05.alloc never waits.
 static_assert(SMEM <= 227 * 1024 && 2 * SMEM > 228 * 1024, "one CTA per SM");
 
@@ -338,21 +433,10 @@ template <int PAGE>
 __global__ void __launch_bounds__(THREADS, 1)
     attend_kernel(const Params p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
-  const int b = blockIdx.z, g = blockIdx.y;
-  int qbeg, nq, ntok, list0;
-  if (!entry_ok(p, b, qbeg, nq, ntok, list0)) return;
-  // the longest rows first: the last queries see the most keys
-  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * (TILES * QT);
-  if (q0 >= nq) return;
-  const int prefix = ntok - nq;
-  const int groups = nq - q0 > QT ? 2 : 1;   // query tiles with a query
-  const Span sp(p, prefix + q0, prefix + min(nq, q0 + TILES * QT) - 1);
-  const int ntiles = sp.ntiles;
-
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = align1024(smem_raw);
   const uint32_t qtile = smem_addr(sm);
-  uint8_t *kring = sm + TILES * TILE, *vring = kring + KS * TILE;
+  uint8_t *kring = sm + QS * TILES * TILE, *vring = kring + KS * TILE;
   Sync* sy = reinterpret_cast<Sync*>(vring + VS * TILE);
   volatile int* abort = &sy->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -363,20 +447,27 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < VS; ++i) {
       mbar_init(&sy->vfull[i], 1);
+      mbar_init(&sy->vclean[i], 1);
       mbar_init(&sy->vempty[i], 1);
+    }
+    for (int i = 0; i < QS; ++i) {
+      mbar_init(&sy->qfull[i], 1);
+      mbar_init(&sy->qempty[i], 1);
+    }
+    for (int i = 0; i < IS; ++i) {
+      mbar_init(&sy->ifull[i], 1);
+      mbar_init(&sy->iempty[i], THREADS / 32 - 1);   // every warp but the load warp
     }
     for (int i = 0; i < TILES; ++i) {
       mbar_init(&sy->sfull[i], 1);
       mbar_init(&sy->sempty[i], SM_WARPS);
       mbar_init(&sy->pfull[i], SM_WARPS);
       mbar_init(&sy->pempty[i], 1);
+      mbar_init(&sy->odone[i], 2);   // an item's last product and the PV thread (the clean warp's notes are in place)
     }
-    mbar_init(&sy->once, 1);
-    mbar_init(&sy->odone, 2);   // the last product and the PV thread (its notes are in place)
     mbar_init(&sy->s_done, 1);
     mbar_init(&sy->pv_done, 1);
     sy->abort = 0;
-    sy->edges = 0;
     fence_mbar_init();
   }
   if (warp == S_WARP) tmem_alloc(&sy->tmem, TMEM_COLS);
@@ -385,35 +476,88 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = sy->tmem;
 
-  if (warp >= K_WARP) {
-    if (warp == K_WARP) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sy->once, groups * TILE);
-        for (int x = 0; x < groups; ++x)
-          tma_load_3d(sm + x * TILE, &qmap, 0, g * GROUP, qbeg + q0 + x * QT, &sy->once);
+  if (warp >= L_WARP) {
+    bool ok = true;
+    Item it;
+    if (warp == L_WARP) {
+      // Chooses this CTA's items (blockIdx.x, + gridDim.x, ...; 32 looked at at a
+      // time) and loads their queries, keys and values.
+      Rings at{kring, vring, sy->kfull, sy->kempty, sy->vfull, sy->vempty, Ring(KS), Ring(VS)};
+      Ring qat(QS);
+      int64_t base = blockIdx.x;
+      unsigned found = 0;
+      for (int i = 0;; ++i) {
+        while (!found && base < p.items) {
+          found = __ballot_sync(0xffffffffu, make_item(p, base + static_cast<int64_t>(lane) * gridDim.x, it));
+          base += 32LL * gridDim.x;
+        }
+        const int from = max(0, __ffs(static_cast<int>(found)) - 1);
+        Item now;
+        now.number = found ? __shfl_sync(0xffffffffu, it.number, from) : p.items;
+        now.g = __shfl_sync(0xffffffffu, it.g, from);
+        now.q0 = __shfl_sync(0xffffffffu, it.q0, from);
+        now.nq = __shfl_sync(0xffffffffu, it.nq, from);
+        now.prefix = __shfl_sync(0xffffffffu, it.prefix, from);
+        now.qbeg = __shfl_sync(0xffffffffu, it.qbeg, from);
+        now.list0 = __shfl_sync(0xffffffffu, it.list0, from);
+        const int s = i % IS, qs = qat.slot;
+        ok = warp_wait_quiet(&sy->iempty[s], ((i / IS) & 1) ^ 1, p.err, abort, lane);
+        if (!ok) break;
+        if (lane == 0) {
+          static_cast<Item&>(sy->items[s]) = now;
+          sy->items[s].edges = 0;
+          mbar_arrive(&sy->ifull[s]);
+        }
+        if (!found) break;
+        found &= found - 1;
+        ok = warp_wait_quiet(&sy->qempty[qs], qat.phase ^ 1, p.err, abort, lane);
+        if (!ok) break;
+        qat.next();
+        if (lane == 0) {
+          const int groups = groups_of(now);
+          mbar_arrive_expect_tx(&sy->qfull[qs], groups * TILE);
+          for (int x = 0; x < groups; ++x)
+            tma_load_3d(sm + (qs * TILES + x) * TILE, &qmap, 0, now.g * GROUP, now.qbeg + now.q0 + x * QT, &sy->qfull[qs]);
+        }
+        __syncwarp();
+        ok = load_tiles<PAGE>(p, span_of(p, now), at, &kmap, &vmap, now.list0, now.g, lane, abort);
+        if (!ok) break;
       }
-      load_tiles<PAGE, KS>(p, sp, &kmap, p.k, kring, sy->kfull, sy->kempty, list0, g, lane, abort);
-      if (lane == 0) mbar_wait(&sy->once, 0, p.err);
-    } else if (warp == V_WARP) {
-      load_tiles<PAGE, VS>(p, sp, &vmap, p.v, vring, sy->vfull, sy->vempty, list0, g, lane, abort);
+      if (!ok) *abort = 1;
+      if (lane == 0) {
+        if (PAGE || p.P >= 8) {
+          drain(sy->kfull, at.k, p.err);
+          drain(sy->vfull, at.v, p.err);
+        }
+        drain(sy->qfull, qat, p.err);
+      }
     } else if (warp == S_WARP) {
       const uint64_t qdesc = sw128_desc(qtile), kdesc = sw128_desc(smem_addr(kring));
-      bool ok = warp_wait_quiet(&sy->once, 0, p.err, abort, lane);
-      int t = 0;
-      for (; t < ntiles && ok; ++t) {
-        const int s = t % KS;
-        ok = warp_wait_quiet(&sy->kfull[s], (t / KS) & 1, p.err, abort, lane);
-        const uint64_t kd = kdesc + static_cast<uint64_t>(s * (TILE >> 4));
-        for (int x = 0; x < groups && ok; ++x) {
-          ok = t == 0 || warp_wait_quiet(&sy->sempty[x], (t - 1) & 1, p.err, abort, lane);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint64_t qd = qdesc + static_cast<uint64_t>(x * (TILE >> 4));
+      Ring k(KS);
+      uint32_t turn = 0;   // bit x: the parity of query tile x's products so far
+      for (int i = 0; next_item(p, sy, i, it, ok, lane); ++i) {
+        release_item(sy, i, lane);
+        const int groups = groups_of(it), ntiles = span_of(p, it).ntiles, qs = i % QS;
+        ok = warp_wait_quiet(&sy->qfull[qs], (i / QS) & 1, p.err, abort, lane);
+        for (int t = 0; t < ntiles && ok; ++t, k.next()) {
+          ok = warp_wait_quiet(&sy->kfull[k.slot], k.phase, p.err, abort, lane);
+          const uint64_t kd = kdesc + static_cast<uint64_t>(k.slot * (TILE >> 4));
+#pragma unroll 1   // (unrolled, here and below, the kernel took 14 % longer)
+          for (int x = 0; x < groups && ok; ++x) {
+            ok = warp_wait_quiet(&sy->sempty[x], ((turn >> x) & 1) ^ 1, p.err, abort, lane);
+            if (!ok) break;
+            turn ^= 1u << x;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint64_t qd = qdesc + static_cast<uint64_t>((qs * TILES + x) * (TILE >> 4));
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) tc_mma(tmem + x * TMEM_TILE, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk > 0);
-            tc_commit(&sy->sfull[x]);
-            if (x + 1 == groups) tc_commit(&sy->kempty[s]);
+              for (int kk = 0; kk < D / 16; ++kk) tc_mma(tmem + x * TMEM_TILE, qd + 2 * kk, kd + 2 * kk, IDESC_S, kk > 0);
+              tc_commit(&sy->sfull[x]);
+              if (x + 1 == groups) {
+                tc_commit(&sy->kempty[k.slot]);
+                if (t + 1 == ntiles) tc_commit(&sy->qempty[qs]);
+              }
+            }
           }
         }
       }
@@ -422,168 +566,209 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_commit(&sy->s_done);   // every product completes before the tensor memory may be freed
         mbar_wait(&sy->s_done, 0, p.err);
       }
+    } else if (warp == C_WARP) {
+      Ring v(VS);
+      for (int i = 0; next_item(p, sy, i, it, ok, lane); ++i) {
+        const Span sp = span_of(p, it);
+        for (int t = 0; t < sp.ntiles && ok; ++t, v.next()) {
+          ok = warp_wait_quiet(&sy->vfull[v.slot], v.phase, p.err, abort, lane);
+          if (!ok) break;
+          if (!sp.whole(sp.key(t))) clean_values(sp, vring + v.slot * TILE, sp.key(t), &sy->items[i % IS], lane);
+          if (lane == 0) mbar_arrive(&sy->vclean[v.slot]);
+        }
+        if (ok) release_item(sy, i, lane);
+      }
+      if (!ok) *abort = 1;
     } else {
       const uint64_t vdesc = sw128_mn_desc(smem_addr(vring));
-      bool ok = true;
-      for (int t = 0; t < ntiles && ok; ++t) {
-        const int s = t % VS;
-        ok = warp_wait_quiet(&sy->vfull[s], (t / VS) & 1, p.err, abort, lane);
-        if (!ok) break;
-        if (!sp.whole(sp.key(t))) clean_values(sp, vring + s * TILE, sp.key(t), sy, lane);
-        const uint64_t vd = vdesc + static_cast<uint64_t>(s * (TILE >> 4));
-        for (int x = 0; x < groups && ok; ++x) {
-          ok = warp_wait_quiet(&sy->pfull[x], t & 1, p.err, abort, lane);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t base = tmem + x * TMEM_TILE;
+      Ring v(VS);
+      uint32_t turn = 0;
+      for (int i = 0; next_item(p, sy, i, it, ok, lane); ++i) {
+        release_item(sy, i, lane);
+        const int groups = groups_of(it), ntiles = span_of(p, it).ntiles;
+        for (int t = 0; t < ntiles && ok; ++t, v.next()) {
+          ok = warp_wait_quiet(&sy->vclean[v.slot], v.phase, p.err, abort, lane);
+          const uint64_t vd = vdesc + static_cast<uint64_t>(v.slot * (TILE >> 4));
+#pragma unroll 1
+          for (int x = 0; x < groups && ok; ++x) {
+            ok = warp_wait_quiet(&sy->pfull[x], (turn >> x) & 1, p.err, abort, lane);
+            if (!ok) break;
+            turn ^= 1u << x;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t base = tmem + x * TMEM_TILE;
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              tc_mma_ts(base + O_COL, base + P_COL + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, t > 0 || kk > 0);
-            tc_commit(&sy->pempty[x]);
-            if (x + 1 == groups) tc_commit(&sy->vempty[s]);
+              for (int kk = 0; kk < BN / 16; ++kk)
+                tc_mma_ts(base + O_COL, base + P_COL + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, t > 0 || kk > 0);
+              tc_commit(&sy->pempty[x]);
+              if (x + 1 == groups) tc_commit(&sy->vempty[v.slot]);
+              if (t + 1 == ntiles) {
+                mbar_arrive(&sy->odone[x]);
+                tc_commit(&sy->odone[x]);
+              }
+            }
           }
         }
       }
       if (lane == 0) {
-        if (ok) {
-          mbar_arrive(&sy->odone);
-          tc_commit(&sy->odone);
-        } else {
-          *abort = 1;
-        }
+        if (!ok) *abort = 1;
         tc_commit(&sy->pv_done);
         mbar_wait(&sy->pv_done, 0, p.err);
       }
     }
     __syncwarp();
-  } else if (warp / SM_WARPS < groups) {
+  } else {
     const int tile = warp / SM_WARPS, quarter = warp & 3, half = (warp >> 2) & 1;
     const int r = quarter * 32 + lane;           // accumulator row = TMEM lane
-    const int q = q0 + tile * QT + r / GROUP;
-    const int h = g * GROUP + r % GROUP;
-    const int pos = prefix + min(q, nq - 1);
     const uint32_t lanes = tmem + tile * TMEM_TILE + (static_cast<uint32_t>(quarter * 32) << 16);
-    // the positions of this warp's rows: a key tile that all of them see in
-    // full needs no mask, whatever the CTA's other rows see
-    Span own = sp;
-    own.p_lo = prefix + min(q0 + tile * QT + quarter * 4, nq - 1);
-    own.p_hi = prefix + min(q0 + tile * QT + quarter * 4 + 3, nq - 1);
     float (&top)[2][2][BM] = sy->top[tile];
-    float m = -INFINITY, l = 0.f;
-    if (groups == 2 && tile == 1) turn_give(0);   // tile 0 begins
-    bool ok = true;   // after a timeout a warp only keeps its partner's barriers
-    for (int t = 0; t < ntiles; ++t) {
-      ok = ok && warp_wait_quiet(&sy->sfull[tile], t & 1, p.err, abort, lane);
-      float mt = -INFINITY;
-      const int k0 = sp.key(t);
-      const bool edge = !own.whole(k0);
-      const uint32_t scol = lanes + half * HALF;
-      // keys of this thread's half that its row sees: i <= hi and (i > lo or i < fi)
-      const int hi = pos - k0 - half * HALF, fi = sp.first - k0 - half * HALF;
-      const int lo = sp.window < 0 || hi < 0 ? -1 : hi - sp.window;
-      // The logits are read twice, 32 at a time, rather than kept: 64 of them do
-      // not fit beside the rest in the 96 registers of a thread among 640.
-      auto logits = [&](int c, float (&v)[32]) {
-        __syncwarp();
-        tmem_ld32(scol + c, v);
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = (c + i <= hi && (c + i > lo || c + i < fi)) ? v[i] : -INFINITY;
-        }
-      };
-      if (ok) {
-        tc_fence_after();
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < HALF; c += 32) {
-          float v[32];
-          logits(c, v);
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[i + 2 * k], v[i + 2 * k + 1]);
-        }
-        mt = p.scale2 * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        top[t & 1][half][r] = mt;
+    uint32_t n = 0, done = 0;                    // this query tile's key tiles and items so far
+    bool ok = true;   // after a timeout a warp only keeps the others' barriers
+    if (tile == 1) turn_give(0);                 // tile 0 begins
+    Item it;
+    it.number = static_cast<int64_t>(blockIdx.x) - gridDim.x;
+    for (int i = 0;; ++i) {
+      if (!next_item(p, sy, i, it, ok, lane)) {
+        if (ok) break;
+        // the items that are left, whose barriers the other warps may be at
+        int64_t number = it.number + gridDim.x;
+        while (number < p.items && !make_item(p, number, it)) number += gridDim.x;
+        if (number >= p.items) break;
       }
-      quarter_sync(tile * 4 + quarter);
-      ok = ok && (t == 0 || warp_wait_quiet(&sy->pempty[tile], (t - 1) & 1, p.err, abort, lane));
-      if (groups == 2) turn_wait(tile);
-      if (!ok) {
-        if (groups == 2 && (tile == 0 || t + 1 < ntiles)) turn_give(tile ^ 1);
-        continue;
-      }
-      mt = fmaxf(mt, top[t & 1][half ^ 1][r]);
-      tc_fence_after();
-      const bool grow = mt > m + LAZY || (m == -INFINITY && mt > -INFINITY);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float mn = grow ? mt : m;
-        const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-        l *= a;
-        m = mn;
-        if (t >= 1) {   // P V(t - 1) has completed: O is at rest; each half takes 32 of its columns
-          __syncwarp();
+      const int groups = groups_of(it);
+      if (tile < groups) {
+        const Span sp = span_of(p, it);
+        const int ntiles = sp.ntiles;
+        const int q = it.q0 + tile * QT + r / GROUP;
+        const int pos = it.prefix + min(q, it.nq - 1);
+        // the positions of this warp's rows: a key tile that all of them see in
+        // full needs no mask, whatever the item's other rows see
+        Span own = sp;
+        own.p_lo = it.prefix + min(it.q0 + tile * QT + quarter * 4, it.nq - 1);
+        own.p_hi = it.prefix + min(it.q0 + tile * QT + quarter * 4 + 3, it.nq - 1);
+        float m = -INFINITY, l = 0.f;
+        for (int t = 0; t < ntiles; ++t, ++n) {
+          ok = ok && warp_wait_quiet(&sy->sfull[tile], n & 1, p.err, abort, lane);
+          float mt = -INFINITY;
+          const int k0 = sp.key(t);
+          const bool edge = !own.whole(k0);
+          const uint32_t scol = lanes + half * HALF;
+          // keys of this thread's half that its row sees: i <= hi and (i > lo or i < fi)
+          const int hi = pos - k0 - half * HALF, fi = sp.first - k0 - half * HALF;
+          const int lo = sp.window < 0 || hi < 0 ? -1 : hi - sp.window;
+          // The logits are read twice, 32 at a time, rather than kept: 64 of them do
+          // not fit beside the rest in the 96 registers of a thread among 640.
+          auto logits = [&](int c, float (&v)[32]) {
+            __syncwarp();
+            tmem_ld32(scol + c, v);
+            if (edge) {
+              const uint32_t see = below(hi + 1 - c) & (~below(lo + 1 - c) | below(fi - c));
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {   // a few columns at a time: the tile's logits stay in registers
-            float o[8];
-            tmem_ld8(lanes + O_COL + half * 32 + c, o);
-            uint32_t w[8];
+              for (int i = 0; i < 32; ++i) v[i] = see & (1u << i) ? v[i] : -INFINITY;
+            }
+          };
+          if (ok) {
+            tc_fence_after();
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(o[i] * a);
-            tmem_st8_async(lanes + O_COL + half * 32 + c, w);
+            for (int c = 0; c < HALF; c += 32) {
+              float v[32];
+              logits(c, v);
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[i + 2 * k], v[i + 2 * k + 1]);
+            }
+            mt = p.scale2 * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            top[n & 1][half][r] = mt;
           }
-        }
-      }
-      const float mu = m == -INFINITY ? 0.f : m;
-      const uint32_t pcol = lanes + P_COL + half * (HALF / 2);
+          quarter_sync(tile * 4 + quarter);
+          ok = ok && warp_wait_quiet(&sy->pempty[tile], (n & 1) ^ 1, p.err, abort, lane);
+          if (groups == 2) turn_wait(tile);
+          if (!ok) {
+            if (groups == 2) turn_give(tile ^ 1);
+            continue;
+          }
+          mt = fmaxf(mt, top[n & 1][half ^ 1][r]);
+          tc_fence_after();
+          const bool grow = mt > m + LAZY || (m == -INFINITY && mt > -INFINITY);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? mt : m;
+            const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            l *= a;
+            m = mn;
+            if (t >= 1) {   // P V(t - 1) has completed: O is at rest; each half takes 32 of its columns
+              __syncwarp();
 #pragma unroll
-      for (int c = 0; c < HALF; c += 32) {
-        float v[32];
-        logits(c, v);
-        if (c + 32 == HALF) {   // S is read: the next product may overwrite it
+              for (int c = 0; c < 32; c += 8) {   // a few columns at a time: the tile's logits stay in registers
+                float o[8];
+                tmem_ld8(lanes + O_COL + half * 32 + c, o);
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(o[i] * a);
+                tmem_st8_async(lanes + O_COL + half * 32 + c, w);
+              }
+            }
+          }
+          const float mu = m == -INFINITY ? 0.f : m;
+          const uint32_t pcol = lanes + P_COL + half * (HALF / 2);
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) {
+            float v[32];
+            logits(c, v);
+            if (c + 32 == HALF) {   // S is read: the next product may overwrite it
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sy->sempty[tile]);
+            }
+            l += weights(v, p.scale2, mu, pcol + c / 2);
+          }
+          if (groups == 2) turn_give(tile ^ 1);
+          tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sy->sempty[tile]);
+          if (lane == 0) mbar_arrive(&sy->pfull[tile]);
         }
-        l += weights(v, p.scale2, mu, pcol + c / 2);
-      }
-      if (groups == 2 && (tile == 0 || t + 1 < ntiles)) turn_give(tile ^ 1);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sy->pfull[tile]);
-    }
-    if (!ok) *abort = 1;
-    top[ntiles & 1][half][r] = l;
-    quarter_sync(tile * 4 + quarter);
-    if (ok && warp_wait_quiet(&sy->odone, 0, p.err, abort, lane)) {
-      l += top[ntiles & 1][half ^ 1][r];
-      tc_fence_after();
-      float o[32];
-      __syncwarp();
-      tmem_ld32(lanes + O_COL + half * 32, o);
-      if (p.sinks) l += exp2f(p.sinks[h] * LOG2E - m);
-      float f = 1.f / l;
-      for (int e = 0; e < min(sy->edges, MAX_EDGE); ++e)
-        for (int w = 0; w < 4; ++w)
-          for (uint32_t bad = sy->edge_bad[e][w]; bad; bad &= bad - 1)
-            if (sp.sees(pos, sy->edge_key[e] + w * 32 + __ffs(bad) - 1)) f = __int_as_float(0x7fc00000);
-      if (q < nq) {
-        uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(qbeg + q) * p.o_st +
-                                              static_cast<int64_t>(h) * p.o_sh + half * 32);
+        // the normaliser, while the last product runs
+        const int h = it.g * GROUP + r % GROUP;
+        const float sink = p.sinks ? p.sinks[h] * LOG2E : -INFINITY;
+        sy->sum[tile][half][r] = l;
+        quarter_sync(tile * 4 + quarter);
+        l += sy->sum[tile][half ^ 1][r];
+        if (p.sinks) l += exp2f(sink - m);
+        float f = 1.f / l;
+        ok = ok && warp_wait_quiet(&sy->odone[tile], done & 1, p.err, abort, lane);
+        ++done;
+        if (ok) {
+          tc_fence_after();
+          float o[32];
+          __syncwarp();
+          tmem_ld32(lanes + O_COL + half * 32, o);
+          const ItemSlot& notes = sy->items[i % IS];
+          for (int e = 0; e < min(notes.edges, MAX_EDGE); ++e)
+            for (int w = 0; w < 4; ++w)
+              for (uint32_t bad = notes.edge_bad[e][w]; bad; bad &= bad - 1)
+                if (sp.sees(pos, notes.edge_key[e] + w * 32 + __ffs(bad) - 1)) f = __int_as_float(0x7fc00000);
+          if (q < it.nq) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(it.qbeg + q) * p.o_st +
+                                                  static_cast<int64_t>(h) * p.o_sh + half * 32);
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
-          uint32_t w[4];
+            for (int c = 0; c < 32; c += 8) {
+              uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(o[c + 2 * i] * f, o[c + 2 * i + 1] * f);
-            w[i] = *reinterpret_cast<const uint32_t*>(&x);
+              for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(o[c + 2 * i] * f, o[c + 2 * i + 1] * f);
+                w[i] = *reinterpret_cast<const uint32_t*>(&x);
+              }
+              dst[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
-          dst[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+      if (ok) release_item(sy, i, lane);
     }
+    if (tile == 0) turn_wait(0);                 // the last turn given
+    if (!ok) *abort = 1;
   }
   tc_fence_before();
   __syncthreads();
@@ -657,6 +842,9 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   p.scale2 = sm_scale * LOG2E;
   p.G = num_kv_heads;
   p.P = page_size;
+  p.bs = bs;
+  p.xs = (max_q + TILES * QT - 1) / (TILES * QT);
+  p.items = static_cast<int64_t>(p.xs) * num_kv_heads * bs;
   p.total_q = total_q;
   p.max_q = max_q;
   p.max_tokens = max_tokens;
@@ -668,7 +856,7 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   p.err = err;
   if (!host::set_smem(attend_kernel<16>, SMEM) || !host::set_smem(attend_kernel<0>, SMEM))
     return host::fail(CE_ERR_CUDA, "ce_window_prefill: smem attr");
-  const dim3 grid((max_q + TILES * QT - 1) / (TILES * QT), num_kv_heads, bs);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.items, host::sm_count()));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (page_size == 16) attend_kernel<16><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
   else attend_kernel<0><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
