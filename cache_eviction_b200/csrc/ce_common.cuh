@@ -388,6 +388,13 @@ __device__ __forceinline__ bool warp_wait_quiet(uint64_t* bar, uint32_t parity, 
   return __shfl_sync(0xffffffffu, ok, 0);
 }
 
+// ---- launches that overlap the end of the one before ------------------------------
+// Lets a launch made with host::launch_after start while this grid still runs.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Returns once every grid this launch depends on has completed and its writes
+// are visible.  (It never waits in a launch that was not made that way.)
+__device__ __forceinline__ void wait_for_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- exponentials ------------------------------------------------------------------
 // 2^x with the SFU's approximate exp2 (PTX ex2.approx.ftz.f32): relative
 // error near 2^-22, -inf -> +0, results below the normal range flush to 0.

@@ -35,6 +35,24 @@ bool set_max_shared_carveout(F* func) {
   return set_max_shared_carveout_attr(reinterpret_cast<const void*>(func));
 }
 
+// A launch that may start while the one before it on the stream still runs, as
+// far as that one's launch_dependents() lets it; its kernel calls
+// wait_for_prerequisites() in every thread before it touches what that one
+// makes.  Errors are left for cudaPeekAtLastError.
+template <class... Args>
+void launch_after(void (*kernel)(Args...), unsigned blocks, unsigned threads, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(threads);
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // Tiled tensor map of `rank` dims (innermost first): dims, byte strides of
 // dims 1..rank-1, box sizes; element strides 1, zero fill out of bounds,
 // 128-byte swizzle or none.
