@@ -41,7 +41,9 @@
 // items are 3.5 rounds of 148.  Short items are bound by their chain of waits
 // (last product, normaliser, output, then the next item's first maximum).
 // (Taking a share of the exponentials as a polynomial on the FMA pipes was
-// slower at every share.)  P in bf16 is rounded by at most 2^-9 of itself, less
+// slower at every share.  So was making a tile's weights with the maximum so
+// far, finding its own beside them, 624 us: the maxima cost little while the
+// product before is still running.)  P in bf16 is rounded by at most 2^-9 of itself, less
 // than the output's own rounding makes of it on average; maxima, sums and O
 // are fp32.
 //
@@ -92,7 +94,7 @@ struct Params {
   const float* sinks;
   float scale2;           // sm_scale * log2(e)
   int G, P;
-  int64_t items;          // query tile pairs x KV heads x entries
+  int64_t items, whole;   // query tile pairs x KV heads x entries; from `whole` on single tiles
   int bs, xs;             // entries, query tile pairs of the longest one
   int total_q, max_q, max_tokens;
   int window, first;
@@ -101,10 +103,10 @@ struct Params {
   int32_t* err;
 };
 
-// One (32 queries, KV head, entry).
+// One (32 or 16 queries, KV head, entry).
 struct Item {
   int64_t number;                 // p.items: no more of them
-  int g, q0, nq, prefix, qbeg, list0;
+  int g, q0, nq, prefix, qbeg, list0;   // queries q0 .. nq - 1, at most 32
 };
 struct ItemSlot : Item {
   int edges;                      // tiles in whose values the clean warp found some that are not finite
@@ -157,10 +159,14 @@ struct Span {
 __device__ __forceinline__ bool make_item(const Params& p, int64_t number, Item& it) {
   if (number >= p.items) return false;
   const int64_t per = static_cast<int64_t>(p.G) * p.bs;
-  const int x = p.xs - 1 - static_cast<int>(number / per), gb = static_cast<int>(number % per), b = gb / p.G;
+  const bool single = number >= p.whole;
+  const int64_t pair = single ? p.whole + (number - p.whole) / 2 : number;
+  const int x = p.xs - 1 - static_cast<int>(pair / per);
+  const int64_t gb = pair % per;
+  const int b = static_cast<int>(gb / p.G);
   it.number = number;
-  it.g = gb % p.G;
-  it.q0 = x * (TILES * QT);
+  it.g = static_cast<int>(gb % p.G);
+  it.q0 = x * (TILES * QT) + (single ? static_cast<int>((number - p.whole) & 1) * QT : 0);
   it.qbeg = p.qo_indptr[b];
   it.nq = p.qo_indptr[b + 1] - it.qbeg;
   it.list0 = p.kv_indptr[b];
@@ -171,11 +177,13 @@ __device__ __forceinline__ bool make_item(const Params& p, int64_t number, Item&
                   ntok <= p.max_tokens && ntok >= it.nq && it.list0 >= 0 && it.list0 + units <= p.kv_capacity &&
                   units <= pages;
   if (!ok && x == 0) flag_error(p.err, CE_EW_SHAPE);
-  return ok && it.q0 < it.nq;
+  const bool some = ok && it.q0 < it.nq;
+  it.nq = min(it.nq, it.q0 + (single ? QT : TILES * QT));
+  return some;
 }
 __device__ __forceinline__ int groups_of(const Item& it) { return it.nq - it.q0 > QT ? 2 : 1; }   // query tiles with a query
 __device__ __forceinline__ Span span_of(const Params& p, const Item& it) {
-  return Span(p, it.prefix + it.q0, it.prefix + min(it.nq, it.q0 + TILES * QT) - 1);
+  return Span(p, it.prefix + it.q0, it.prefix + it.nq - 1);
 }
 
 // A position in a ring of n slots and the parity of its round.  (A wait for the
@@ -844,7 +852,18 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   p.P = page_size;
   p.bs = bs;
   p.xs = (max_q + TILES * QT - 1) / (TILES * QT);
+  // A last round that would leave half of the SMs or more without an item is
+  // given out as single query tiles, which take a CTA about 0.87 of a pair's time
+  // (64 queries behind 26,624 tokens 132 -> 115 us, 256 of them 134 -> 119 us, the
+  // chunk of the header, whose last round has 68 items, 542 -> 538 us).
+  const int sms = host::sm_count();
   p.items = static_cast<int64_t>(p.xs) * num_kv_heads * bs;
+  p.whole = p.items;
+  const int64_t rest = p.items % sms;
+  if (2 * rest <= sms) {
+    p.whole -= rest;
+    p.items += rest;
+  }
   p.total_q = total_q;
   p.max_q = max_q;
   p.max_tokens = max_tokens;
@@ -856,7 +875,7 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   p.err = err;
   if (!host::set_smem(attend_kernel<16>, SMEM) || !host::set_smem(attend_kernel<0>, SMEM))
     return host::fail(CE_ERR_CUDA, "ce_window_prefill: smem attr");
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.items, host::sm_count()));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.items, sms));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (page_size == 16) attend_kernel<16><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
   else attend_kernel<0><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);

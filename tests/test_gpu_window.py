@@ -334,3 +334,10 @@ def test_chunk_bad_entries_are_flagged_and_left():
     idx[5] = pools.shape[1]
     flag, out = run(csr=(csr[0], idx, csr[2]))
     assert flag == capi.CE_EW_INDEX and torch.equal(out[:10], good[:10])
+
+
+@pytest.mark.parametrize("G,lens", [(1, [33, 16, 17, 1, 0, 64, 15]), (8, [600, 31, 0, 601]), (2, [2400, 7])])
+def test_chunk_items_of_pairs_and_single_tiles(G, lens):
+    """Batches whose query tiles are all single ones, whole rounds of pairs, and
+    pairs with a last round of single ones, with empty entries among them."""
+    check_chunk([(n, 40 * (i % 3)) for i, n in enumerate(lens)], G, 16, 50, 4, seed=91 + G)
