@@ -497,7 +497,9 @@ int ce_kv4_read(const void* k_pool, const void* v_pool, int64_t pool_units, cons
  * Arguments, scores and score_flags (CE_SCORE_DEFER too, with
  * ce_decode_scores afterwards) as there, except that kv_tokens is required,
  * the output is bf16, sm_scale is positive and score_sg >= pool_units.  Slots
- * beyond a row's tokens may hold anything.
+ * beyond a row's tokens may hold anything.  A page of a scored row belongs to
+ * that row alone: of two rows that add to one score in a call, one addition
+ * may be lost (attention itself may share pages).
  * Supported: head_dim 64, H/G == 8, G 1, 2, 4 or 8, page_size 16. */
 int64_t ce_kv4_decode_workspace_bytes(int32_t bs, int64_t kv_capacity, int32_t num_q_heads,
                                       int32_t num_kv_heads, int32_t score_flags);
