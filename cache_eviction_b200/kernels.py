@@ -8,6 +8,7 @@ calls allocate nothing.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Sequence
 
@@ -205,12 +206,13 @@ def _on(device: torch.device, *tensors) -> None:
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(fn, name: str, device: torch.device, *args) -> None:
     """fn(*args, stream) on `device`'s current stream, with `device` current."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         st = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -219,13 +221,11 @@ def _call(fn, name: str, device: torch.device, *args) -> None:
         capi.check(st, name)
 
 
-def _bytes(fn, name: str, device: torch.device, *args) -> int:
-    """A workspace query on `device` (the sizes go by its multiprocessors)."""
-    if torch.cuda.current_device() == device.index:
-        need = fn(*args)
-    else:
-        with torch.cuda.device(device.index):
-            need = fn(*args)
+@functools.lru_cache(maxsize=1024)
+def _bytes(name: str, index: int, *args) -> int:
+    """A workspace query on device `index` (the sizes go by its multiprocessors)."""
+    with torch.cuda.device(index):
+        need = getattr(capi.load(), name)(*args)
     if need < 0:
         raise capi.CeError(f"{name} failed")
     return need
@@ -265,9 +265,11 @@ def _queries(q: torch.Tensor, align: int) -> torch.Tensor:
     return q.clone(memory_format=torch.contiguous_format)
 
 
-def _output(out, shape, device, *dtypes) -> torch.Tensor:
+def _output(out, q, *dtypes) -> torch.Tensor:
+    """The caller's output for q [a, b, 64], or a new one of the first dtype."""
     if out is None:
-        return torch.empty(shape, dtype=dtypes[0], device=device)
+        return torch.empty_like(q, dtype=dtypes[0], memory_format=torch.contiguous_format)
+    shape = q.shape
     if out.dtype not in dtypes or out.shape != shape or (out.numel() and out.stride(2) != 1):
         _bad(f"out must be {' or '.join(map(str, dtypes))} {list(shape)} with dense rows")
     return out
@@ -333,15 +335,15 @@ def kv4_read(k_pool, v_pool, units, k_out=None, v_out=None, err=None):
         _bad("units must be dense int32 [n]")
     n = units.numel()
     dev = k_pool.device
-    shape = torch.Size((n, G, 16, 64))
-    if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    shape = (n, G, 16, 64)
     for t in (k_out, v_out):
-        if t.dtype != torch.bfloat16 or t.shape != shape or (n and t.stride(3) != 1):
+        if t is not None and (t.dtype != torch.bfloat16 or t.shape != shape or (n and t.stride(3) != 1)):
             _bad(f"outputs must be bf16 {list(shape)} with dense rows")
     _on(dev, k_pool, v_pool, units, k_out, v_out, err)
+    if k_out is None:
+        k_out = k_pool.new_empty(shape, dtype=torch.bfloat16)
+    if v_out is None:
+        v_out = k_pool.new_empty(shape, dtype=torch.bfloat16)
     ku, kg, kt, _ = k_out.stride()
     vu, vg, vt, _ = v_out.stride()
     _call(lib.ce_kv4_read, "ce_kv4_read", dev, _at(k_pool), _at(v_pool), pool_units, _at(units), n, G, 64, 16,
@@ -362,7 +364,8 @@ def kv4_decode_attn_score(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, s
                           score_flags=3, err=None, workspace=None):
     """Fused decode attention + H2O score over one layer's 4-bit pages
     (ce_kv4_decode_attn_score): decode_attn_score with pools from kv4_pool,
-    16-token pages and a bf16 output.  capi.CE_SCORE_DEFER in score_flags
+    16-token pages and a bf16 output.  Pages of scored rows are not shared
+    between rows (unscored ones may be).  capi.CE_SCORE_DEFER in score_flags
     leaves the page scores to decode_scores, from the workspace then given."""
     lib = capi.load()
     units, G = _kv4_pools(k_pool, v_pool)
@@ -370,7 +373,7 @@ def kv4_decode_attn_score(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, s
     bs, H, D = q.shape
     dev = q.device
     _csr(kv_indptr, kv_indices, kv_tokens, bs)
-    out = _output(out, q.shape, dev, torch.bfloat16)
+    out = _output(out, q, torch.bfloat16)
     _lse(lse, bs * H)
     score_sg = 0
     if scores is not None:
@@ -390,7 +393,7 @@ def kv4_decode_attn_score(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, s
     cap = kv_indices.numel()
     if scores is None or mode_of_row is None:
         score_flags &= ~3          # nothing to score: no room for it either
-    need = _bytes(lib.ce_kv4_decode_workspace_bytes, "ce_kv4_decode_workspace_bytes", dev, bs, cap, H, G, score_flags)
+    need = _bytes("ce_kv4_decode_workspace_bytes", dev.index, bs, cap, H, G, score_flags)
     ws = _workspace(need, workspace, dev)
     _call(lib.ce_kv4_decode_attn_score, "ce_kv4_decode_attn_score", dev, _at(q), q.stride(0), q.stride(1), _at(k_pool),
           _at(v_pool), units, _at(kv_indptr), _at(kv_indices), _at(kv_tokens), cap, _at(sinks), _at(mode_of_row),
@@ -421,12 +424,12 @@ def window_decode(q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sm_scale,
     bs, H, D = q.shape
     dev = q.device
     _csr(kv_indptr, kv_indices, kv_tokens, bs)
-    out = _output(out, q.shape, dev, *((torch.float32, torch.bfloat16) if out_f32 else (torch.bfloat16, torch.float32)))
+    out = _output(out, q, *((torch.float32, torch.bfloat16) if out_f32 else (torch.bfloat16, torch.float32)))
     _lse(lse, bs * H)
     _on(dev, q, k_pool, v_pool, kv_indptr, kv_indices, kv_tokens, sinks, out, lse, err)
     sinks = _sinks(sinks, H)
     cap = kv_indices.numel()
-    need = _bytes(lib.ce_decode_workspace_bytes, "ce_decode_workspace_bytes", dev, bs, cap, H, G, page_size, 0)
+    need = _bytes("ce_decode_workspace_bytes", dev.index, bs, cap, H, G, page_size, 0)
     ws = _workspace(need, workspace, dev)
     _call(lib.ce_window_decode, "ce_window_decode", dev, _at(q), q.stride(0), q.stride(1), _at(k_pool), _at(v_pool),
           units, _at(kv_indptr), _at(kv_indices), _at(kv_tokens), cap, _at(sinks), sm_scale, bs, H, G, D, page_size,
@@ -454,7 +457,7 @@ def window_prefill(q, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_token
     _csr(kv_indptr, kv_indices, kv_tokens, bs)
     if qo_indptr.dtype != torch.int32 or not qo_indptr.is_contiguous() or qo_indptr.numel() < bs + 1:
         _bad("qo_indptr must hold one more dense int32 than there are entries")
-    out = _output(out, q.shape, dev, torch.bfloat16)
+    out = _output(out, q, torch.bfloat16)
     _on(dev, q, k_pool, v_pool, qo_indptr, kv_indptr, kv_indices, kv_tokens, sinks, out, err)
     sinks = _sinks(sinks, H)
     _call(lib.ce_window_prefill, "ce_window_prefill", dev, _at(q), q.stride(0), q.stride(1), _at(k_pool), _at(v_pool),
