@@ -30,14 +30,14 @@
 // an item's loads, first products and clean-up run under the one before.  (A CTA
 // per item left the SM idle while it started and ended: 207 us instead of 123
 // for prompts of 4,093 and 3,069 tokens, 64 heads, window 128, where an item
-// has two key tiles.)
+// has two key tiles; 110 with the clean warp's loop rolled.)
 // The exponentials bound long items (one per row and key on a unit of 16 per
 // clock and SM: 2,048 clocks per key tile and item, against 1,536 of the tensor
 // cores), so the two query tiles take turns at them: while one computes its
 // weights the other's waits, reads and maxima go on.  Left to themselves (two
 // CTAs per SM) the tiles fell into step, both at the exponentials and then both
 // waiting.  2,048 queries behind 26,624 tokens (2,048 first + 6,144 window), 64
-// heads: 540 us, 509 TFLOP/s, ~4,000 clocks per key tile and item; its 512
+// heads: 494 us, 557 TFLOP/s, ~3,600 clocks per key tile and item; its 512
 // items are 3.5 rounds of 148.  Short items are bound by their chain of waits
 // (last product, normaliser, output, then the next item's first maximum).
 // (Taking a share of the exponentials as a polynomial on the FMA pipes was
@@ -335,13 +335,13 @@ __device__ __forceinline__ void clean_values(const Span& sp, uint8_t* tile, int 
   uint8_t* mine = tile + (lane >> 3) * 128 + (lane & 7) * 16;
   const int row0 = lane >> 3, end = sp.p_hi + 1 - k, from = sp.lo - k, head = sp.first - k;
   uint32_t acc[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1   // (unrolled it took 9 % of the whole kernel: its instructions evict the softmax warps')
+  for (int i0 = 0; i0 < BN / 4; i0 += 4) {
+    uint4 x[4];
 #pragma unroll
-  for (int i0 = 0; i0 < BN / 4; i0 += 8) {
-    uint4 x[8];
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(mine + (i0 + i) * 512);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(mine + (i0 + i) * 512);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int row = (i0 + i) * 4 + row0;
       if (row >= end || (row < from && row >= head)) {   // no query sees it
         *reinterpret_cast<uint4*>(mine + (i0 + i) * 512) = make_uint4(0u, 0u, 0u, 0u);
@@ -356,27 +356,24 @@ __device__ __forceinline__ void clean_values(const Span& sp, uint8_t* tile, int 
   __syncwarp();
   const uint32_t found = not_finite(acc[0]) | not_finite(acc[1]) | not_finite(acc[2]) | not_finite(acc[3]);
   if (__any_sync(0xffffffffu, found != 0u)) {
-    uint32_t bad[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
+#pragma unroll 1
     for (int w = 0; w < 4; ++w) {
+      uint32_t bad = 0u;
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
-        const int row = w * 32 + i * 4;
-        uint4* at = reinterpret_cast<uint4*>(mine + row * 128);
-        uint4 x = *at;
+        uint4* at = reinterpret_cast<uint4*>(mine + (w * 32 + i * 4) * 128);
+        const uint4 x = *at;
         const uint4 nf = make_uint4(not_finite(x.x), not_finite(x.y), not_finite(x.z), not_finite(x.w));
         if (nf.x | nf.y | nf.z | nf.w) {
           *at = make_uint4(x.x & ~nf.x, x.y & ~nf.y, x.z & ~nf.z, x.w & ~nf.w);
-          bad[w] |= 1u << (i * 4 + (lane >> 3));
+          bad |= 1u << (i * 4 + (lane >> 3));
         }
       }
+      bad = __reduce_or_sync(0xffffffffu, bad);
+      if (lane == 0 && e < MAX_EDGE) it->edge_bad[e][w] = bad;
     }
-#pragma unroll
-    for (int w = 0; w < 4; ++w) bad[w] = __reduce_or_sync(0xffffffffu, bad[w]);
     if (lane == 0 && e < MAX_EDGE) {
       it->edge_key[e] = k;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) it->edge_bad[e][w] = bad[w];
       it->edges = e + 1;
     }
   }
@@ -707,7 +704,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             m = mn;
             if (t >= 1) {   // P V(t - 1) has completed: O is at rest; each half takes 32 of its columns
               __syncwarp();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < 32; c += 8) {   // a few columns at a time: the tile's logits stay in registers
                 float o[8];
                 tmem_ld8(lanes + O_COL + half * 32 + c, o);
@@ -855,7 +852,8 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   // A last round that would leave half of the SMs or more without an item is
   // given out as single query tiles, which take a CTA about 0.87 of a pair's time
   // (64 queries behind 26,624 tokens 132 -> 115 us, 256 of them 134 -> 119 us, the
-  // chunk of the header, whose last round has 68 items, 542 -> 538 us).
+  // chunk of the header, whose last round has 68 items, 542 -> 538 us, before the
+  // clean warp's loop was rolled).
   const int sms = host::sm_count();
   p.items = static_cast<int64_t>(p.xs) * num_kv_heads * bs;
   p.whole = p.items;
