@@ -341,3 +341,32 @@ def test_chunk_items_of_pairs_and_single_tiles(G, lens):
     """Batches whose query tiles are all single ones, whole rounds of pairs, and
     pairs with a last round of single ones, with empty entries among them."""
     check_chunk([(n, 40 * (i % 3)) for i, n in enumerate(lens)], G, 16, 50, 4, seed=91 + G)
+
+
+def test_chunk_is_repeatable_on_two_streams_at_once():
+    """Many items per CTA, replayed from two captured graphs on two streams:
+    every run gives the same bits."""
+    from cache_eviction_b200 import kernels
+    gen = torch.Generator().manual_seed(17)
+    made = []
+    for parts, G, window, first in (([(700, 60), (33, 500), (1, 0), (0, 9), (1200, 0)], 8, 100, 20), ([(300, 2000)], 2, -1, 0)):
+        pools, _, csr, _, _ = batch([a + b for a, b in parts], G, 16, gen)
+        nqs = [a for a, _ in parts]
+        ptr = torch.tensor([0] + nqs).cumsum(0).to(torch.int32).to(DEV)
+        q = torch.randn((sum(nqs), 8 * G, 64), generator=gen).to(torch.bfloat16).to(DEV)
+        a = (q, pools[0].to(DEV), pools[1].to(DEV), ptr, *csr, SCALE, 16, max(nqs), max(a + b for a, b in parts), window)
+        want = kernels.window_prefill(*a, first=first)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = kernels.window_prefill(*a, first=first)
+        made.append((graph, out, want, a))
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(40):
+        for (graph, out, _, _), st in zip(made, streams):
+            with torch.cuda.stream(st):
+                out.fill_(math.nan)
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in made:
+            assert torch.equal(out, want)
