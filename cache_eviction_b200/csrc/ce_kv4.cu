@@ -51,17 +51,16 @@ __device__ __forceinline__ void encode(const uint32_t (&w)[4], float lo, float s
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   const uint64_t minus = pair(-lo, -lo), by = pair(inv, inv), magic = pair(MAGIC, MAGIC), back = pair(-MAGIC, -MAGIC);
-  bool tie = false;
+  float off = 0.f;   // the largest distance from a code
   uint32_t r[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint64_t t = mul2(add2(pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), minus), by);
-    const uint64_t m = add2(t, magic), c = add2(m, back);
-    float t0, t1, c0, c1, m0, m1;
-    split(t, t0, t1);
-    split(c, c0, c1);
+    const uint64_t m = add2(t, magic);
+    float d0, d1, m0, m1;
+    split(fma2(add2(m, back), pair(-1.f, -1.f), t), d0, d1);
     split(m, m0, m1);
-    tie = tie || fabsf(t0 - c0) > 0.49999f || fabsf(t1 - c1) > 0.49999f;
+    off = max3(off, fabsf(d0), fabsf(d1));
     r[2 * i] = __float_as_uint(m0);
     r[2 * i + 1] = __float_as_uint(m1);
   }
@@ -75,7 +74,7 @@ __device__ __forceinline__ void encode(const uint32_t (&w)[4], float lo, float s
     }
     return;
   }
-  if (tie) {
+  if (off > 0.49999f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       r[2 * i] = settle(__uint_as_float(r[2 * i]), __uint_as_float(w[i] << 16) - lo, s);
@@ -91,7 +90,7 @@ __device__ __forceinline__ void encode(const uint32_t (&w)[4], float lo, float s
 // aligned quads of a page (the first token's slot gives the phase); a whole
 // quad's V bytes are gathered into words and stored as 128 consecutive bytes,
 // any other set of slots byte by byte.  29,719 tokens of 8 heads take about
-// 34 us (76 MB): bound by the issue slots (70 %) and the ALU (62 %), most of it
+// 33 us (76 MB): bound by the issue slots (70 %) and the ALU (62 %), most of it
 // rounding, packing and exchanging codes.
 __global__ void __launch_bounds__(THREADS) write_kernel(const WriteParams p) {
   const int lane = threadIdx.x & 31, l = lane & 7, jq = lane >> 3;
