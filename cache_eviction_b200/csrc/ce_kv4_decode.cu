@@ -16,11 +16,13 @@
 // exactly.  One 32-bit word of codes is a whole m16n8k16 A fragment of V, or
 // two K-steps' halves of K, for four ANDs and a shift.  The other operand
 // brings the range back: the query row is scaled by a power of two to
-// 2^14 .. 2^15 (1/16 of that where it meets upper nibbles), and the weights
-// p_t s_t by 2^15 over a power of two above every scale seen so far (in the
-// exponent of p_t itself), so both are ordinary fp16 numbers.  Rounding them to fp16 (2^-12 relative at most,
-// 2^-39 of the largest) is far below the output's bf16 rounding; logits,
-// maxima, sums and accumulators are fp32.
+// 2^14 .. 2^15 (1/16 of that where it meets upper nibbles), and a head's weights
+// p_t s_t by a power of two, 2^lift, that puts the largest of them so far at
+// 2^9 or above and below 2^16, so both are ordinary fp16 numbers.  (The lift
+// goes by p_t s_t, not by the scales alone: a row of large values that a head
+// does not look at must not push the others out of fp16.)  Rounding p_t s_t to
+// fp16 costs at most 2^-11 of it, or 2^-34 of the largest where it falls below
+// fp16's normal range; logits, maxima, sums and accumulators are fp32.
 //
 // A producer warp copies whole pages (all KV heads) into a ring of shared-memory
 // stages with untiled bulk copies; the format puts a page's fragments in lane
@@ -52,7 +54,7 @@ constexpr int PPW = 2;                               // pages that a warp comput
 constexpr int CTAS_PER_SM = 2;
 constexpr int MIN_STAGES_LOG2 = 0;                   // every CTA below min(stages, grid) has one
 
-// Floats of a record: the unnormalised outputs [H][64], then (maximum, sum) [H].
+// Floats of a record: the means of V [H][64], then (maximum, sum of p) [H].
 __host__ __device__ constexpr int rec_floats(int H) { return H * (D + 2); }
 
 // D += A(16x16) * B(16x8) in fp16 with fp32 accumulation.
@@ -88,25 +90,27 @@ constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 struct Rows {
   uint32_t qb[4][2];    // B operand of S^T: query codes' partners, fp16
   float qs0, qs1;       // 2^-24 sum of the scaled query row
-  float kq0, kq1;       // log2-domain logit of u = s (q . c) + m sum q
   float o[4][4];        // rows r + 8 hold sum w s (16 hi), rows r the sum of both halves
-  float m0, m1;         // running maxima rounded up to integers (NO_MAX: none yet), the same in a head's lanes
-  float bound, lift;    // a power of two above every V scale so far; log2(2^15 / bound)
-  uint64_t kq, nm;      // (kq0, kq1); (lift - m0, lift - m1): a weight is w = 2^(u kq + nm) = p 2^lift
-  uint64_t l;           // this lane's sums of w
   float z0, z1;         // this lane's sums of w m
+  // pairs, of head 2t and head 2t + 1:
+  uint64_t kq;          // u kq is the logit in log2 units, u = s (q . c) + m sum q
+  uint64_t nm;          // minus a recent maximum of the logits, rounded up to an integer (NO_MAX: none yet), the same in a head's lanes
+  uint64_t f;           // 2^lift: w = p 2^lift, p = 2^(u kq - m); every w s so far is below 2^16
+  uint64_t l;           // this lane's sums of p
 };
 
-constexpr float NO_MAX = -1e30f;                      // below every logit that is not -inf
-constexpr float MIN_BOUND = 8.077935669463161e-28f;   // 2^-90: 2^lift stays far from fp32's end
+constexpr float NO_MAX = -1e30f;   // below every logit that is not -inf
+constexpr int TOP = 15, SLACK = 5;   // w s may reach 2^TOP; where it could pass that, room of 2^SLACK is made
+constexpr int MAX_LIFT = 105, MAX_P = 100;   // logs of what 2^lift, w and p may reach: sums stay far from fp32's end
+// A row of one value has scale 0: 2^-60 of its minimum counts as its scale, so that
+// w m stays below 2^76.  (A scale that is not 0 is at least 2^-12 of the minimum.)
+constexpr float OF_MIN = 8.673617379884035e-19f;
 
 __device__ __forceinline__ void clear(Rows& s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) s.o[i][0] = s.o[i][1] = s.o[i][2] = s.o[i][3] = 0.f;
-  s.m0 = s.m1 = NO_MAX;
-  s.bound = MIN_BOUND;
-  s.lift = 105.f;
   s.nm = pair(-NO_MAX, -NO_MAX);
+  s.f = pair(pow2_bits(127 + MAX_LIFT), pow2_bits(127 + MAX_LIFT));
   s.l = pair(0.f, 0.f);
   s.z0 = s.z1 = 0.f;
 }
@@ -147,9 +151,7 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
   const float kq = scale_log2 * pow2_bits(min(ex + 10, 254));  // 2^24 / f
   s.qs0 = __shfl_sync(0xffffffffu, qs, 8 * t);
   s.qs1 = __shfl_sync(0xffffffffu, qs, 8 * t + 4);
-  s.kq0 = __shfl_sync(0xffffffffu, kq, 8 * t);
-  s.kq1 = __shfl_sync(0xffffffffu, kq, 8 * t + 4);
-  s.kq = pair(s.kq0, s.kq1);
+  s.kq = pair(__shfl_sync(0xffffffffu, kq, 8 * t), __shfl_sync(0xffffffffu, kq, 8 * t + 4));
 }
 
 // Untiled bulk copy of `bytes` (a multiple of 16) into shared memory.
@@ -166,6 +168,74 @@ struct Side {           // where a scored sequence's page data goes
   int H, hcol;          // this lane's first head
   float *ul, *tl;
 };
+
+// What counts as the scale of a token (or the largest of several) from its (scale, |minimum|).
+__device__ __forceinline__ float reach(__nv_bfloat162 par) { return fmaxf(__low2float(par), __high2float(par) * OF_MIN); }
+__device__ __forceinline__ __nv_bfloat162 magnitudes(uint32_t par) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&par)); }
+
+// log2 of a power of two.
+__device__ __forceinline__ float log2_of(float pow2) { return static_cast<float>(static_cast<int>(__float_as_uint(pow2) >> 23) - 127); }
+
+// The running state moved so that the maxima cover x0 kq and x1 kq (this lane's
+// largest logits) and every w s of the tile (logits u kq, V parameters vp) is at
+// most 2^(TOP - SLACK).
+__device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const uint2 (&vp)[PPW], float x0, float x1) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+  }
+  float kq0, kq1, m0, m1, f0, f1;
+  split(s.kq, kq0, kq1);
+  x0 *= kq0;
+  x1 *= kq1;
+  split(s.nm, m0, m1);
+  split(s.f, f0, f1);
+  m0 = -m0;
+  m1 = -m1;
+  const float n0 = fmaxf(m0, ceilf(x0)), n1 = fmaxf(m1, ceilf(x1));
+  const float lift0 = log2_of(f0), lift1 = log2_of(f1);
+  float r0 = -INFINITY, r1 = -INFINITY;   // log2 of the tile's largest p s
+#pragma unroll
+  for (int i = 0; i < 2 * PPW; ++i) {
+    const float e = __log2f(reach(magnitudes(i & 1 ? vp[i / 2].y : vp[i / 2].x)));
+    r0 = fmaxf(r0, u[i / 2][2 * (i & 1)] * kq0 - n0 + e);
+    r1 = fmaxf(r1, u[i / 2][2 * (i & 1) + 1] * kq1 - n1 + e);
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+    r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, o));
+    r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, o));
+  }
+  // What was added before is below 2^(TOP + m - n) now; the lift may rise again by as much.
+  const float t0 = fminf(fminf(lift0 + (n0 - m0), static_cast<float>(MAX_LIFT)), floorf(static_cast<float>(TOP - SLACK) - r0));
+  const float t1 = fminf(fminf(lift1 + (n1 - m1), static_cast<float>(MAX_LIFT)), floorf(static_cast<float>(TOP - SLACK) - r1));
+  // Sums of p go by 2^(m - n), sums of w by 2^(m - n + change of the lift), which
+  // may be further from 1 than an fp32 is though the product is not: in steps.
+  float d0 = m0 - n0, d1 = m1 - n1;
+  float l0, l1;
+  split(s.l, l0, l1);
+  s.l = pair(l0 * fast_exp2(d0), l1 * fast_exp2(d1));
+  d0 = fmaxf(d0 + (t0 - lift0), -300.f);
+  d1 = fmaxf(d1 + (t1 - lift1), -300.f);
+  s.nm = pair(-n0, -n1);
+  s.f = pair(fast_exp2(t0), fast_exp2(t1));
+#pragma unroll 1
+  do {
+    const float a0 = fast_exp2(fmaxf(d0, -100.f)), a1 = fast_exp2(fmaxf(d1, -100.f));
+    s.z0 *= a0;
+    s.z1 *= a1;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s.o[q][0] *= a0;
+      s.o[q][1] *= a1;
+      s.o[q][2] *= a0;
+      s.o[q][3] *= a1;
+    }
+    d0 = fminf(d0 + 100.f, 0.f);
+    d1 = fminf(d1 + 100.f, 0.f);
+  } while (__any_sync(0xffffffffu, d0 < 0.f || d1 < 0.f));
+}
 
 // PPW pages (the first `ntok` tokens of them) of KV head g: K slices at kb,
 // V slices at vb, one page every `stride` bytes.
@@ -194,51 +264,30 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     u[pg][2] = vb2 ? fmaf(sb, c[2], mb * s.qs0) : -INFINITY;
     u[pg][3] = vb2 ? fmaf(sb, c[3], mb * s.qs1) : -INFINITY;
   }
-  // V scales and minima, and what could move the running state: a logit above
-  // its head's maximum, or a V scale at or above the bound.
+  // V scales and minima, and what moves the running state: a logit and a scale
+  // (not always of one token) that could take a w s beyond 2^TOP.  A logit above
+  // the maximum so far does not: p may pass 1 until then.
   uint2 vp[PPW];
-  float x0 = -INFINITY, x1 = -INFINITY, top = 0.f;
+  float x0 = -INFINITY, x1 = -INFINITY;
+  __nv_bfloat162 top = __float2bfloat162_rn(pow2_bits(127 + TOP - MAX_LIFT));   // so that w itself stays below 2^MAX_LIFT
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     vp[pg] = *reinterpret_cast<const uint2*>(vb + pg * stride + CODE_BYTES + r * 8);
     if (TAIL && pg * P + 2 * r >= ntok) vp[pg].x = 0u;
     if (TAIL && pg * P + 2 * r + 1 >= ntok) vp[pg].y = 0u;
-    top = max3(top, __uint_as_float(vp[pg].x << 16), __uint_as_float(vp[pg].y << 16));
+    top = __hmax2(top, __hmax2(magnitudes(vp[pg].x), magnitudes(vp[pg].y)));
     x0 = max3(x0, u[pg][0], u[pg][2]);
     x1 = max3(x1, u[pg][1], u[pg][3]);
   }
-  if (__any_sync(0xffffffffu, x0 * s.kq0 > s.m0 || x1 * s.kq1 > s.m1 || top >= s.bound)) {
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    const float n0 = fmaxf(s.m0, ceilf(x0 * s.kq0)), n1 = fmaxf(s.m1, ceilf(x1 * s.kq1));
-    float f = 1.f;
-    if (top >= s.bound) {   // the same for every lane
-      const float nb = pow2_bits(min(static_cast<int>(__float_as_uint(top) >> 23) + 1, 253));
-      f = s.bound * (1.f / nb);
-      s.bound = nb;
-      s.lift = static_cast<float>(15 + 127 - static_cast<int>(__float_as_uint(nb) >> 23));
-    }
-    const float a0 = fast_exp2(s.m0 - n0) * f, a1 = fast_exp2(s.m1 - n1) * f;
-    s.m0 = n0;
-    s.m1 = n1;
-    s.nm = pair(s.lift - n0, s.lift - n1);
-    float l0, l1;
-    split(s.l, l0, l1);
-    s.l = pair(l0 * a0, l1 * a1);
-    s.z0 *= a0;
-    s.z1 *= a1;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s.o[q][0] *= a0;
-      s.o[q][1] *= a1;
-      s.o[q][2] *= a0;
-      s.o[q][3] *= a1;
-    }
+  {
+    float a0, a1, f0, f1;
+    split(fma2(pair(x0, x1), s.kq, s.nm), a0, a1);
+    split(s.f, f0, f1);
+    if (__any_sync(0xffffffffu, fmaxf(a0, a1) + fmaxf(__log2f(reach(top) * fmaxf(f0, f1)), TOP - MAX_P) > TOP))
+      move(s, u, vp, x0, x1);
   }
+  float kq0, kq1;   // MODE MAX
+  split(s.kq, kq0, kq1);
   float mass[2 * PPW];   // MODE SUM: this lane's share of the pages' masses, heads 2t and 2t + 1
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
@@ -250,6 +299,8 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     const uint64_t both = add2(pair(e[0], e[1]), pair(e[2], e[3]));
     s.l = add2(s.l, both);
     if (MODE == CE_MODE_SUM) split(both, mass[2 * pg], mass[2 * pg + 1]);
+    split(mul2(pair(e[0], e[1]), s.f), e[0], e[1]);
+    split(mul2(pair(e[2], e[3]), s.f), e[2], e[3]);
     const float sa = __uint_as_float(vp[pg].x << 16), ma = __uint_as_float(vp[pg].x & 0xffff0000u);
     const float sb = __uint_as_float(vp[pg].y << 16), mb = __uint_as_float(vp[pg].y & 0xffff0000u);
     s.z0 = fmaf(e[0], ma, fmaf(e[2], mb, s.z0));
@@ -271,7 +322,7 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
         const int j = 2 * r + h;
         if ((!TAIL || pg * P + j < ntok) && side.cpos + pg < side.capacity)
           *reinterpret_cast<float2*>(side.tl + ((side.cpos + pg) * P + j) * side.H + side.hcol) =
-              make_float2(u[pg][2 * h] * s.kq0, u[pg][2 * h + 1] * s.kq1);
+              make_float2(u[pg][2 * h] * kq0, u[pg][2 * h + 1] * kq1);
       }
     }
   }
@@ -319,11 +370,11 @@ __device__ __forceinline__ void stage(Rows& s, const uint8_t* kb, const uint8_t*
   }
 }
 
-// The warp's sums over its lanes, and its output row in place: head 2t of dims
-// 16 q + r (i = 0) and 16 q + r + 8 (i = 2), head 2t + 1 likewise (i = 1, 3).
+// The warp's sums over its lanes, and in place of the accumulators the means of
+// V that its weights make (which no range of values takes beyond fp32, as sums
+// could be): head 2t of dims 16 q + r (i = 0) and 16 q + r + 8 (i = 2), head
+// 2t + 1 likewise (i = 1, 3).
 __device__ __forceinline__ void finish(Rows& s, float& l0, float& l1) {
-  // sums hold w = p 2^lift; the accumulators w s (c 2^-24), upper nibbles 16-fold
-  const float down = pow2_bits(127 - static_cast<int>(s.lift));
   split(s.l, l0, l1);
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
@@ -332,19 +383,18 @@ __device__ __forceinline__ void finish(Rows& s, float& l0, float& l1) {
     s.z0 += __shfl_xor_sync(0xffffffffu, s.z0, o);
     s.z1 += __shfl_xor_sync(0xffffffffu, s.z1, o);
   }
-  l0 *= down;
-  l1 *= down;
-  s.z0 *= down;
-  s.z1 *= down;
+  // accumulators hold w s (c 2^-24), upper nibbles 16-fold; w = p 2^lift
+  float f0, f1;
+  split(s.f, f0, f1);
+  const float d0 = fast_exp2(-log2_of(f0)), d1 = fast_exp2(-log2_of(f1));
+  const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    s.o[q][0] = fmaf((s.o[q][0] - s.o[q][2]) * 16777216.f, down, s.z0);
-    s.o[q][1] = fmaf((s.o[q][1] - s.o[q][3]) * 16777216.f, down, s.z1);
-    s.o[q][2] = fmaf(s.o[q][2] * 1048576.f, down, s.z0);
-    s.o[q][3] = fmaf(s.o[q][3] * 1048576.f, down, s.z1);
+    s.o[q][0] = fmaf(s.o[q][0] - s.o[q][2], 16777216.f, s.z0) * i0 * d0;
+    s.o[q][1] = fmaf(s.o[q][1] - s.o[q][3], 16777216.f, s.z1) * i1 * d1;
+    s.o[q][2] = fmaf(s.o[q][2], 1048576.f, s.z0) * i0 * d0;
+    s.o[q][3] = fmaf(s.o[q][3], 1048576.f, s.z1) * i1 * d1;
   }
-  if (s.m0 == NO_MAX) s.m0 = -INFINITY;
-  if (s.m1 == NO_MAX) s.m1 = -INFINITY;
 }
 
 // A warp's heads into rows h0 .. h0 + 7 of a record-shaped buffer of H heads.
@@ -360,9 +410,11 @@ __device__ __forceinline__ void put(const Rows& s, float l0, float l1, float* re
   }
   if (r == 0) {
     float* ml = rec + H * D + (h0 + 2 * t) * 2;
-    ml[0] = s.m0;
+    float m0, m1;
+    split(s.nm, m0, m1);
+    ml[0] = m0 == -NO_MAX ? -INFINITY : -m0;
     ml[1] = l0;
-    ml[2] = s.m1;
+    ml[2] = m1 == -NO_MAX ? -INFINITY : -m1;
     ml[3] = l1;
   }
 }
@@ -387,22 +439,25 @@ __device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp,
   consumers_sync();
   for (int i = threadIdx.x; i < H * D / 2; i += NW * 32) {
     const int h = i / (D / 2);
-    float m[SUB], top = -INFINITY;
+    float w[SUB], top = -INFINITY, l = 0.f;
 #pragma unroll
     for (int k = 0; k < SUB; ++k) {
-      m[k] = part[k * rec_floats(H) + H * D + 2 * h];
-      top = fmaxf(top, m[k]);
+      w[k] = part[k * rec_floats(H) + H * D + 2 * h];
+      top = fmaxf(top, w[k]);
     }
-    float2 o = make_float2(0.f, 0.f);
-    float l = 0.f;
 #pragma unroll
     for (int k = 0; k < SUB; ++k) {
-      const float* q = part + k * rec_floats(H);
-      const float w = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - top);
-      const float2 x = reinterpret_cast<const float2*>(q)[i];
-      o.x += w * x.x;
-      o.y += w * x.y;
-      l += w * q[H * D + 2 * h + 1];
+      w[k] = w[k] == -INFINITY ? 0.f : fast_exp2(w[k] - top);
+      w[k] *= part[k * rec_floats(H) + H * D + 2 * h + 1];
+      l += w[k];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < SUB; ++k) {
+      const float2 x = reinterpret_cast<const float2*>(part + k * rec_floats(H))[i];
+      o.x = fmaf(w[k] * inv, x.x, o.x);
+      o.y = fmaf(w[k] * inv, x.y, o.y);
     }
     reinterpret_cast<float2*>(rec)[i] = o;
     if (i % (D / 2) == 0) {
@@ -717,14 +772,17 @@ __global__ void __launch_bounds__(CB_THREADS) combine_kernel(const Params p, int
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     top = fmaxf(top, m);
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-    float sum = w * ml.y;
+    float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+    w *= ml.y;
+    float sum = w;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    const float a = m == -INFINITY ? 0.f : exp2f(m - top);
-    l = l * a + sum;
-    o.x *= a;
-    o.y *= a;
+    const float before = l * (m == -INFINITY ? 0.f : exp2f(m - top));
+    l = before + sum;
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // o stays a mean
+    o.x *= before * inv;
+    o.y *= before * inv;
+    w *= inv;
     m = top;
     for (int i0 = 0; i0 < cnt; i0 += 8) {
       float2 v[8];
@@ -755,15 +813,21 @@ __global__ void __launch_bounds__(CB_THREADS) combine_kernel(const Params p, int
     m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < W; ++k) m = fmaxf(m, sh_ml[k][0]);
+    float w[W];
     l = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      w[k] = sh_ml[k][0] == -INFINITY ? 0.f : exp2f(sh_ml[k][0] - m);
+      w[k] *= sh_ml[k][1];
+      l += w[k];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     o = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-      const float a = sh_ml[k][0] == -INFINITY ? 0.f : exp2f(sh_ml[k][0] - m);
       const float2 x = reinterpret_cast<const float2*>(sh_o[k])[lane];
-      l += a * sh_ml[k][1];
-      o.x = fmaf(a, x.x, o.x);
-      o.y = fmaf(a, x.y, o.y);
+      o.x = fmaf(w[k] * inv, x.x, o.x);
+      o.y = fmaf(w[k] * inv, x.y, o.y);
     }
   }
   // with the sink in the normaliser; a row with neither tokens nor a sink is
@@ -772,8 +836,8 @@ __global__ void __launch_bounds__(CB_THREADS) combine_kernel(const Params p, int
   const float top = fmaxf(m, sink2);
   float L = -INFINITY, f = 0.f;
   if (n > 0 || sink2 != -INFINITY) {
-    const float a = m == -INFINITY ? (l != l ? l : 0.f) : exp2f(m - top);   // a row of NaN logits has no maximum
-    const float den = l * a + (p.sinks ? exp2f(sink2 - top) : 0.f);
+    const float a = l * (m == -INFINITY ? (l != l ? l : 0.f) : exp2f(m - top));   // a row of NaN logits has no maximum
+    const float den = a + (p.sinks ? exp2f(sink2 - top) : 0.f);
     L = top + log2f(den);
     f = a / den;
   }

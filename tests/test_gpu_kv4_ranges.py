@@ -1,0 +1,142 @@
+"""4-bit decode attention where the ranges of fp32 and fp16 could end: value
+rows of one value, scales far apart, rows that nobody looks at, logits of any
+magnitude, query rows near the largest bf16, and long rows in one block.
+
+Everything is held to attention over the same pages in 64 bits.  Tolerances,
+from the arithmetic, as in test_gpu_kv4.py: a logit is off by at most
+d = 80 * 2^-24 * scale * (s sum |q| c + |m| sum |q|), a p by the relative
+e = 2 d + 16 * 2^-24 * (1 + |logit range|); p s is rounded to fp16 (2^-11
+relative; below fp16's normal range 2^-25, where the largest p s of the row is
+at least 2^9, so 2^-34 of that one); the output to bf16 (2^-8):
+
+    |error| <= 2^-8 |o| + (2^-11 + e) sum p s c + (e + A 2^-24) sum p |m|
+               + 2^-34 n 15 max(p s)
+
+with A the additions that a term of sum p m goes through (at most n / 8 in a
+lane and 64 after that).
+"""
+import math
+
+import pytest
+import torch
+
+import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+SCALE = 0.125
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from cache_eviction_b200 import capi
+    capi.load()
+
+
+def slices(x, is_key):
+    """Tokens x [n, G, 64] bf16 as pages [ceil(n / 16), G, 576] (the rest of the last page zeros)."""
+    n, G = x.shape[:2]
+    full = torch.zeros((-(-n // 16) * 16, G, 64), dtype=torch.bfloat16)
+    full[:n] = x
+    return ref.pack(*ref.quantise(full.view(-1, 16, G, 64).transpose(1, 2)), is_key)
+
+
+def one_row(q, kp, vp, n, sinks=None):
+    """The operator over one row of n tokens in pages 0, 1, ... -> out [H, 64], lse [H] (64 bits, host)."""
+    from cache_eviction_b200 import kernels
+    units, G = kp.shape[:2]
+    i32 = dict(dtype=torch.int32, device=DEV)
+    lse, err = torch.empty((1, 8 * G), device=DEV), torch.zeros(1, **i32)
+    out = kernels.kv4_decode_attn_score(q[None].to(DEV), kp.to(DEV), vp.to(DEV), torch.tensor([0, units], **i32),
+                                        torch.arange(units, **i32), torch.tensor([n], **i32), SCALE,
+                                        sinks=None if sinks is None else sinks.to(DEV), lse=lse, err=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    return out[0].double().cpu(), lse[0].double().cpu()
+
+
+def hold(q, kp, vp, n):
+    """one_row against the 64-bit form, every head."""
+    out, lse = one_row(q, kp, vp, n)
+    for g in range(kp.shape[1]):
+        (kc, ks, km), (vc, vs, vm) = ((x.reshape(-1, x.shape[-1])[:n] for x in ref.unpack(t[:, g], key))
+                                      for t, key in ((kp, True), (vp, False)))
+        hs = slice(8 * g, 8 * g + 8)
+        qq = q[hs].double()
+        p, o, l = ref.attend(qq[None], km + kc * ks, vm + vc * vs, torch.ones(1, n, dtype=torch.bool), None, SCALE)
+        p, o, l = p[0], o[0], l[0]
+        d = 80 * 2.0 ** -24 * SCALE * (qq.abs() @ kc.T * ks.T + qq.abs().sum(-1, keepdim=True) * km.abs().T).amax(-1)
+        logits = qq @ (km + kc * ks).T * SCALE
+        e = (2 * d + 16 * 2.0 ** -24 * (1 + (logits - l[:, None]).abs().amax(-1)))[:, None]
+        assert (e < 0.25).all()      # a tolerance that tells something
+        tol = (2.0 ** -8 * o.abs() + (2.0 ** -11 + e) * (p @ (vc * vs)) + (e + (n / 8 + 64) * 2.0 ** -24) * (p @ vm.abs())
+               + 2.0 ** -34 * n * 15 * (p * vs.T).amax(-1, keepdim=True) + 1e-37)
+        assert ((out[hs] - o).abs() <= tol).all(), (g, float(((out[hs] - o).abs() / tol).nan_to_num(1e9).max()))
+        assert ((lse[hs] - l).abs() <= e[:, 0] + 2.0 ** -22 * (1 + l.abs())).all()
+
+
+def draws(n, G, seed):
+    gen = torch.Generator().manual_seed(seed)
+    k = (torch.randn((n, G, 64), generator=gen) + 0.5 * torch.randn((1, G, 64), generator=gen)).to(torch.bfloat16)
+    v = torch.randn((n, G, 64), generator=gen)
+    return (torch.randn((8 * G, 64), generator=gen) * 1.5).to(torch.bfloat16), k, v
+
+
+# ------------------------------------------------------------ value rows of one value
+@pytest.mark.parametrize("G", [1, 8])
+@pytest.mark.parametrize("n", [1, 700, 70003])
+@pytest.mark.parametrize("value", [0.0, 1.0, 3e3, 1e7, -1e7, 1e30, -3e38])
+def test_value_rows_of_one_value(value, n, G):
+    """Every value row is constant (scale 0): the output is that value.  Its
+    terms p m and the sum of p pass through at most n / 8 + 64 additions each."""
+    q, k, _ = draws(n, G, n + G)
+    v = torch.full((n, G, 64), value, dtype=torch.bfloat16)
+    out, _ = one_row(q, slices(k, True), slices(v, False), n)
+    want = v.double()[0, 0, 0]
+    tol = (2.0 ** -8 + 2 * (n / 8 + 64) * 2.0 ** -24) * want.abs()
+    assert ((out - want).abs() <= tol).all(), out
+
+
+@pytest.mark.parametrize("G,n", [(1, 700), (8, 700), (2, 20011)])
+@pytest.mark.parametrize("value", [0.0, 1e4, -1e7, 1e30])
+@pytest.mark.parametrize("spread", [1.0, 2.0 ** 60, 2.0 ** 110])
+def test_constant_rows_before_and_after_others(value, spread, G, n):
+    """What came before counts, however far the scales that follow are from its."""
+    q, k, v = draws(n, G, 3)
+    kp = slices(k, True)
+    for some in (slice(0, n // 2 + 3), slice(n // 2 + 3, n)):
+        x = v * spread
+        x[some] = value
+        hold(q, kp, slices(x.to(torch.bfloat16), False), n)
+
+
+@pytest.mark.parametrize("G", [1, 8])
+@pytest.mark.parametrize("power", [20, 40, 100])
+@pytest.mark.parametrize("at", [0, 350, 699])
+def test_a_large_value_row_that_heads_do_not_see(at, power, G):
+    """One value row is 2^power times the others; half of the heads give it a
+    weight near 0 and keep the others' contributions, half see little else."""
+    n = 700
+    q, k, v = draws(n, G, 5)
+    sign = torch.tensor([1.0, -1.0]).repeat(4 * G)
+    q[:, :8] = (4 * sign[:, None]).to(torch.bfloat16)
+    k[:, :, :8] = 0
+    k[at] = 0
+    k[at, :, :8] = -40.0                       # logits of 8 * 4 * 40 / 8 = 160, down or up
+    v[at] *= 2.0 ** power
+    hold(q, slices(k, True), slices(v.to(torch.bfloat16), False), n)
+
+
+@pytest.mark.parametrize("G,n", [(1, 700), (8, 2011)])
+@pytest.mark.parametrize("zeros", [0, 300, 690, 10 ** 6])
+@pytest.mark.parametrize("rise", [-400.0, 40.0, 400.0])
+def test_logits_that_rise_or_fall_along_a_row(rise, zeros, G, n):
+    """Logits that change by `rise` over the row, its first value rows zeros:
+    weights of rows that add nothing grow as well."""
+    q, k, v = draws(n, G, 6)
+    q[:, :8] = 4.0
+    k[:, :, :8] = (rise / 4.0 * (torch.arange(n) / n - 0.5)).view(-1, 1, 1)     # logit 4 * 8 / 8 of it
+    v[:zeros] = 0.0
+    hold(q, slices(k, True), slices(v.to(torch.bfloat16), False), n)
