@@ -18,10 +18,10 @@
 // brings the range back: the query row is scaled by a power of two to
 // 2^14 .. 2^15 (1/16 of that where it meets upper nibbles), and a head's weights
 // p_t s_t by a power of two, 2^lift, that puts the largest of them so far at
-// 2^9 or above and below 2^16, so both are ordinary fp16 numbers.  (The lift
+// 2^7 or above and below 2^16, so both are ordinary fp16 numbers.  (The lift
 // goes by p_t s_t, not by the scales alone: a row of large values that a head
 // does not look at must not push the others out of fp16.)  Rounding p_t s_t to
-// fp16 costs at most 2^-11 of it, or 2^-34 of the largest where it falls below
+// fp16 costs at most 2^-11 of it, or 2^-32 of the largest where it falls below
 // fp16's normal range; logits, maxima, sums and accumulators are fp32.
 //
 // A producer warp copies whole pages (all KV heads) into a ring of shared-memory
@@ -90,27 +90,38 @@ constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 struct Rows {
   uint32_t qb[4][2];    // B operand of S^T: query codes' partners, fp16
   float qs0, qs1;       // 2^-24 sum of the scaled query row
-  float o[4][4];        // rows r + 8 hold sum w s (16 hi), rows r the sum of both halves
+  float o[4][4];        // sums of w s c 2^-24 (rows r), of w s 16 c 2^-24 (rows r + 8)
   float z0, z1;         // this lane's sums of w m
-  // pairs, of head 2t and head 2t + 1:
+  // pairs, of head 2t and head 2t + 1, the same in a head's lanes:
   uint64_t kq;          // u kq is the logit in log2 units, u = s (q . c) + m sum q
-  uint64_t nm;          // minus a recent maximum of the logits, rounded up to an integer (NO_MAX: none yet), the same in a head's lanes
-  uint64_t f;           // 2^lift: w = p 2^lift, p = 2^(u kq - m); every w s so far is below 2^16
-  uint64_t l;           // this lane's sums of p
+  uint64_t nm;          // minus a recent maximum of the logits, rounded up to an integer (NO_MAX: none yet)
+  uint64_t lift;        // w = p 2^lift, p = 2^(u kq - m); every w s so far is below 2^16
+  uint64_t l;           // this lane's sums of w
+  __nv_bfloat162 bound; // V scales and magnitudes of minima up to here are taken with p up to 2^ROOM_P
 };
 
-constexpr float NO_MAX = -1e30f;   // below every logit that is not -inf
-constexpr int TOP = 15, SLACK = 5;   // w s may reach 2^TOP; where it could pass that, room of 2^SLACK is made
-constexpr int MAX_LIFT = 105, MAX_P = 100;   // logs of what 2^lift, w and p may reach: sums stay far from fp32's end
-// A row of one value has scale 0: 2^-60 of its minimum counts as its scale, so that
+constexpr float NO_MAX = -1e30f;     // below every logit that is not -inf
+// log2 of what w s may reach, of how far p may pass 1 and a scale the one that
+// the lift was chosen by before it is chosen again, and of what 2^lift may reach
+// (sums of w stay far from fp32's end).
+constexpr int TOP = 15, ROOM_P = 3, ROOM_S = 4, MAX_LIFT = 105;
+// A row of one value has scale 0: 2^OF_MIN of its minimum counts as its scale, so that
 // w m stays below 2^76.  (A scale that is not 0 is at least 2^-12 of the minimum.)
-constexpr float OF_MIN = 8.673617379884035e-19f;
+constexpr int OF_MIN = -60;
+
+// The bound that goes with the larger of a lane's two lifts.
+__device__ __forceinline__ __nv_bfloat162 bound_of(float lift) {
+  const int e = 127 + TOP - ROOM_P - static_cast<int>(lift);
+  const uint32_t b = static_cast<uint32_t>(min(e, 255) << 7 | min(e - OF_MIN, 255) << 23);   // (infinite from 2^128 on)
+  return *reinterpret_cast<const __nv_bfloat162*>(&b);
+}
 
 __device__ __forceinline__ void clear(Rows& s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) s.o[i][0] = s.o[i][1] = s.o[i][2] = s.o[i][3] = 0.f;
   s.nm = pair(-NO_MAX, -NO_MAX);
-  s.f = pair(pow2_bits(127 + MAX_LIFT), pow2_bits(127 + MAX_LIFT));
+  s.lift = pair(MAX_LIFT, MAX_LIFT);
+  s.bound = bound_of(MAX_LIFT);
   s.l = pair(0.f, 0.f);
   s.z0 = s.z1 = 0.f;
 }
@@ -169,36 +180,33 @@ struct Side {           // where a scored sequence's page data goes
   float *ul, *tl;
 };
 
-// What counts as the scale of a token (or the largest of several) from its (scale, |minimum|).
-__device__ __forceinline__ float reach(__nv_bfloat162 par) { return fmaxf(__low2float(par), __high2float(par) * OF_MIN); }
 __device__ __forceinline__ __nv_bfloat162 magnitudes(uint32_t par) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&par)); }
 
-// log2 of a power of two.
-__device__ __forceinline__ float log2_of(float pow2) { return static_cast<float>(static_cast<int>(__float_as_uint(pow2) >> 23) - 127); }
+constexpr float REST = TOP - ROOM_P - ROOM_S;
 
 // The running state moved so that the maxima cover x0 kq and x1 kq (this lane's
 // largest logits) and every w s of the tile (logits u kq, V parameters vp) is at
-// most 2^(TOP - SLACK).
+// most 2^REST.
 __device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const uint2 (&vp)[PPW], float x0, float x1) {
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
     x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
   }
-  float kq0, kq1, m0, m1, f0, f1;
+  float kq0, kq1, m0, m1, lift0, lift1;
   split(s.kq, kq0, kq1);
   x0 *= kq0;
   x1 *= kq1;
   split(s.nm, m0, m1);
-  split(s.f, f0, f1);
+  split(s.lift, lift0, lift1);
   m0 = -m0;
   m1 = -m1;
   const float n0 = fmaxf(m0, ceilf(x0)), n1 = fmaxf(m1, ceilf(x1));
-  const float lift0 = log2_of(f0), lift1 = log2_of(f1);
   float r0 = -INFINITY, r1 = -INFINITY;   // log2 of the tile's largest p s
 #pragma unroll
   for (int i = 0; i < 2 * PPW; ++i) {
-    const float e = __log2f(reach(magnitudes(i & 1 ? vp[i / 2].y : vp[i / 2].x)));
+    const uint32_t par = i & 1 ? vp[i / 2].y : vp[i / 2].x;
+    const float e = __log2f(fmaxf(__uint_as_float(par << 16), fabsf(__uint_as_float(par & 0xffff0000u)) * pow2_bits(127 + OF_MIN)));
     r0 = fmaxf(r0, u[i / 2][2 * (i & 1)] * kq0 - n0 + e);
     r1 = fmaxf(r1, u[i / 2][2 * (i & 1) + 1] * kq1 - n1 + e);
   }
@@ -208,21 +216,18 @@ __device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const ui
     r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, o));
   }
   // What was added before is below 2^(TOP + m - n) now; the lift may rise again by as much.
-  const float t0 = fminf(fminf(lift0 + (n0 - m0), static_cast<float>(MAX_LIFT)), floorf(static_cast<float>(TOP - SLACK) - r0));
-  const float t1 = fminf(fminf(lift1 + (n1 - m1), static_cast<float>(MAX_LIFT)), floorf(static_cast<float>(TOP - SLACK) - r1));
-  // Sums of p go by 2^(m - n), sums of w by 2^(m - n + change of the lift), which
-  // may be further from 1 than an fp32 is though the product is not: in steps.
-  float d0 = m0 - n0, d1 = m1 - n1;
-  float l0, l1;
-  split(s.l, l0, l1);
-  s.l = pair(l0 * fast_exp2(d0), l1 * fast_exp2(d1));
-  d0 = fmaxf(d0 + (t0 - lift0), -300.f);
-  d1 = fmaxf(d1 + (t1 - lift1), -300.f);
+  const float t0 = fminf(fminf(lift0 + (n0 - m0), static_cast<float>(MAX_LIFT)), floorf(REST - r0));
+  const float t1 = fminf(fminf(lift1 + (n1 - m1), static_cast<float>(MAX_LIFT)), floorf(REST - r1));
+  // The sums go by 2^(m - n + change of the lift), which may be further from 1
+  // than an fp32 is though their products with it are not: in steps.
+  float d0 = fmaxf(m0 - n0 + (t0 - lift0), -300.f), d1 = fmaxf(m1 - n1 + (t1 - lift1), -300.f);
   s.nm = pair(-n0, -n1);
-  s.f = pair(fast_exp2(t0), fast_exp2(t1));
+  s.lift = pair(t0, t1);
+  s.bound = bound_of(fmaxf(t0, t1));
 #pragma unroll 1
   do {
     const float a0 = fast_exp2(fmaxf(d0, -100.f)), a1 = fast_exp2(fmaxf(d1, -100.f));
+    s.l = mul2(s.l, pair(a0, a1));
     s.z0 *= a0;
     s.z1 *= a1;
 #pragma unroll
@@ -264,67 +269,75 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     u[pg][2] = vb2 ? fmaf(sb, c[2], mb * s.qs0) : -INFINITY;
     u[pg][3] = vb2 ? fmaf(sb, c[3], mb * s.qs1) : -INFINITY;
   }
-  // V scales and minima, and what moves the running state: a logit and a scale
-  // (not always of one token) that could take a w s beyond 2^TOP.  A logit above
-  // the maximum so far does not: p may pass 1 until then.
+  // V scales and minima, and what moves the running state: a logit or a scale
+  // with which a w s could pass 2^TOP.
   uint2 vp[PPW];
   float x0 = -INFINITY, x1 = -INFINITY;
-  __nv_bfloat162 top = __float2bfloat162_rn(pow2_bits(127 + TOP - MAX_LIFT));   // so that w itself stays below 2^MAX_LIFT
+  __nv_bfloat162 top = s.bound;
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     vp[pg] = *reinterpret_cast<const uint2*>(vb + pg * stride + CODE_BYTES + r * 8);
     if (TAIL && pg * P + 2 * r >= ntok) vp[pg].x = 0u;
     if (TAIL && pg * P + 2 * r + 1 >= ntok) vp[pg].y = 0u;
-    top = __hmax2(top, __hmax2(magnitudes(vp[pg].x), magnitudes(vp[pg].y)));
+    top = __hmax2(__hmax2(top, magnitudes(vp[pg].x)), magnitudes(vp[pg].y));
     x0 = max3(x0, u[pg][0], u[pg][2]);
     x1 = max3(x1, u[pg][1], u[pg][3]);
   }
   {
-    float a0, a1, f0, f1;
+    float a0, a1;
     split(fma2(pair(x0, x1), s.kq, s.nm), a0, a1);
-    split(s.f, f0, f1);
-    if (__any_sync(0xffffffffu, fmaxf(a0, a1) + fmaxf(__log2f(reach(top) * fmaxf(f0, f1)), TOP - MAX_P) > TOP))
+    if (__any_sync(0xffffffffu, fmaxf(a0, a1) > ROOM_P || *reinterpret_cast<const uint32_t*>(&top) != *reinterpret_cast<const uint32_t*>(&s.bound)))
       move(s, u, vp, x0, x1);
   }
-  float kq0, kq1;   // MODE MAX
-  split(s.kq, kq0, kq1);
+  if (MODE == CE_MODE_MAX) {
+    float kq0, kq1;
+    split(s.kq, kq0, kq1);
+#pragma unroll
+    for (int i = 0; i < 2 * PPW; ++i) {
+      const int pg = i / 2, h = i & 1, j = 2 * r + h;
+      if ((!TAIL || pg * P + j < ntok) && side.cpos + pg < side.capacity)
+        *reinterpret_cast<float2*>(side.tl + ((side.cpos + pg) * P + j) * side.H + side.hcol) =
+            make_float2(u[pg][2 * h] * kq0, u[pg][2 * h + 1] * kq1);
+    }
+  }
+  uint32_t pt[PPW][2];   // w s in fp16, as B operands of O^T
   float mass[2 * PPW];   // MODE SUM: this lane's share of the pages' masses, heads 2t and 2t + 1
+  const uint64_t base = add2(s.nm, s.lift);
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     float e[4];
-    split(fma2(pair(u[pg][0], u[pg][1]), s.kq, s.nm), e[0], e[1]);
-    split(fma2(pair(u[pg][2], u[pg][3]), s.kq, s.nm), e[2], e[3]);
+    split(fma2(pair(u[pg][0], u[pg][1]), s.kq, base), e[0], e[1]);
+    split(fma2(pair(u[pg][2], u[pg][3]), s.kq, base), e[2], e[3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = fast_exp2(e[i]);
     const uint64_t both = add2(pair(e[0], e[1]), pair(e[2], e[3]));
     s.l = add2(s.l, both);
     if (MODE == CE_MODE_SUM) split(both, mass[2 * pg], mass[2 * pg + 1]);
-    split(mul2(pair(e[0], e[1]), s.f), e[0], e[1]);
-    split(mul2(pair(e[2], e[3]), s.f), e[2], e[3]);
     const float sa = __uint_as_float(vp[pg].x << 16), ma = __uint_as_float(vp[pg].x & 0xffff0000u);
     const float sb = __uint_as_float(vp[pg].y << 16), mb = __uint_as_float(vp[pg].y & 0xffff0000u);
     s.z0 = fmaf(e[0], ma, fmaf(e[2], mb, s.z0));
     s.z1 = fmaf(e[1], ma, fmaf(e[3], mb, s.z1));
-    const uint32_t p0 = movmatrix_trans(pack_f16(e[0] * sa, e[1] * sa));
-    const uint32_t p1 = movmatrix_trans(pack_f16(e[2] * sb, e[3] * sb));
-    const uint4 w = *reinterpret_cast<const uint4*>(vb + pg * stride + (t * 8 + r) * 16);
-    const uint32_t wq[4] = {w.x, w.y, w.z, w.w};
+    pt[pg][0] = movmatrix_trans(pack_f16(e[0] * sa, e[1] * sa));
+    pt[pg][1] = movmatrix_trans(pack_f16(e[2] * sb, e[3] * sb));
+  }
+  // The tensor cores cut what they add to 24 bits of the largest term, always
+  // towards 0, which over thousands of positive terms is a drift: they add up
+  // one tile's, and the tiles are added in fp32.
+  uint4 wv[PPW];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      // rows r take a byte's both codes, lo + 16 hi, rows r + 8 its 16 hi alone:
-      // finish() subtracts (the weights are the same, so exactly up to fp32)
-      const uint32_t even = __byte_perm(wq[q], 0u, 0x4240), odd = __byte_perm(wq[q], 0u, 0x4341);
-      mma_f16(s.o[q], even, even & HIGH, odd, odd & HIGH, p0, p1);
-    }
-    if (MODE == CE_MODE_MAX) {
+  for (int pg = 0; pg < PPW; ++pg) wv[pg] = *reinterpret_cast<const uint4*>(vb + pg * stride + (t * 8 + r) * 16);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int j = 2 * r + h;
-        if ((!TAIL || pg * P + j < ntok) && side.cpos + pg < side.capacity)
-          *reinterpret_cast<float2*>(side.tl + ((side.cpos + pg) * P + j) * side.H + side.hcol) =
-              make_float2(u[pg][2 * h] * kq0, u[pg][2 * h + 1] * kq1);
-      }
+  for (int q = 0; q < 4; ++q) {
+    float c[4];
+#pragma unroll
+    for (int pg = 0; pg < PPW; ++pg) {
+      const uint32_t w = q == 0 ? wv[pg].x : q == 1 ? wv[pg].y : q == 2 ? wv[pg].z : wv[pg].w;
+      const uint32_t odd = w >> 8;
+      if (pg == 0) mma_f16_zero(c, w & LOW, w & HIGH, odd & LOW, odd & HIGH, pt[pg][0], pt[pg][1]);
+      else mma_f16(c, w & LOW, w & HIGH, odd & LOW, odd & HIGH, pt[pg][0], pt[pg][1]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.o[q][i] += c[i];
   }
   if (MODE == CE_MODE_SUM) {
     // Sum the 4 (page, head) shares over the lanes of equal t; each step halves
@@ -343,7 +356,7 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     const int pg = r >> 2, h = (r >> 1) & 1;
     if (!(r & 1) && (!TAIL || pg * P < ntok) && side.cpos + pg < side.capacity) {
       float n0, n1;
-      split(s.nm, n0, n1);
+      split(base, n0, n1);
       side.ul[(side.cpos + pg) * side.H + side.hcol + h] = y > 0.f ? __log2f(y) - (h ? n1 : n0) : -INFINITY;
     }
   }
@@ -370,11 +383,12 @@ __device__ __forceinline__ void stage(Rows& s, const uint8_t* kb, const uint8_t*
   }
 }
 
-// The warp's sums over its lanes, and in place of the accumulators the means of
-// V that its weights make (which no range of values takes beyond fp32, as sums
-// could be): head 2t of dims 16 q + r (i = 0) and 16 q + r + 8 (i = 2), head
-// 2t + 1 likewise (i = 1, 3).
-__device__ __forceinline__ void finish(Rows& s, float& l0, float& l1) {
+// The warp's sums of p over its lanes and the means of V that its weights make
+// (which no range of values takes beyond fp32, as sums could be), into rows
+// h0 .. h0 + 7 of a record-shaped buffer of H heads.
+__device__ __forceinline__ void put(Rows& s, float* rec, int H, int h0, int lane) {
+  const int r = lane >> 2, t = lane & 3;
+  float l0, l1, m0, m1, lift0, lift1;
   split(s.l, l0, l1);
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
@@ -383,39 +397,23 @@ __device__ __forceinline__ void finish(Rows& s, float& l0, float& l1) {
     s.z0 += __shfl_xor_sync(0xffffffffu, s.z0, o);
     s.z1 += __shfl_xor_sync(0xffffffffu, s.z1, o);
   }
-  // accumulators hold w s (c 2^-24), upper nibbles 16-fold; w = p 2^lift
-  float f0, f1;
-  split(s.f, f0, f1);
-  const float d0 = fast_exp2(-log2_of(f0)), d1 = fast_exp2(-log2_of(f1));
+  split(s.nm, m0, m1);
+  split(s.lift, lift0, lift1);
   const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    s.o[q][0] = fmaf(s.o[q][0] - s.o[q][2], 16777216.f, s.z0) * i0 * d0;
-    s.o[q][1] = fmaf(s.o[q][1] - s.o[q][3], 16777216.f, s.z1) * i1 * d1;
-    s.o[q][2] = fmaf(s.o[q][2], 1048576.f, s.z0) * i0 * d0;
-    s.o[q][3] = fmaf(s.o[q][3], 1048576.f, s.z1) * i1 * d1;
-  }
-}
-
-// A warp's heads into rows h0 .. h0 + 7 of a record-shaped buffer of H heads.
-__device__ __forceinline__ void put(const Rows& s, float l0, float l1, float* rec, int H, int h0, int lane) {
-  const int r = lane >> 2, t = lane & 3;
   float* o = rec + (h0 + 2 * t) * D + r;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    o[q * 16] = s.o[q][0];
-    o[D + q * 16] = s.o[q][1];
-    o[q * 16 + 8] = s.o[q][2];
-    o[D + q * 16 + 8] = s.o[q][3];
+    o[q * 16] = fmaf(s.o[q][0], 16777216.f, s.z0) * i0;
+    o[D + q * 16] = fmaf(s.o[q][1], 16777216.f, s.z1) * i1;
+    o[q * 16 + 8] = fmaf(s.o[q][2], 1048576.f, s.z0) * i0;
+    o[D + q * 16 + 8] = fmaf(s.o[q][3], 1048576.f, s.z1) * i1;
   }
   if (r == 0) {
     float* ml = rec + H * D + (h0 + 2 * t) * 2;
-    float m0, m1;
-    split(s.nm, m0, m1);
     ml[0] = m0 == -NO_MAX ? -INFINITY : -m0;
-    ml[1] = l0;
+    ml[1] = l0 * fast_exp2(-lift0);
     ml[2] = m1 == -NO_MAX ? -INFINITY : -m1;
-    ml[3] = l1;
+    ml[3] = l1 * fast_exp2(-lift1);
   }
 }
 
@@ -428,14 +426,12 @@ template <int G>
 __device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp, int lane, float* part) {
   constexpr int H = G * GROUP, SUB = NW / G;
   float* rec = p.rec + static_cast<int64_t>(b + blockIdx.x) * rec_floats(H);
-  float l0, l1;
-  finish(s, l0, l1);
   if constexpr (SUB == 1) {
-    put(s, l0, l1, rec, H, warp * GROUP, lane);
+    put(s, rec, H, warp * GROUP, lane);
     return;
   }
   consumers_sync();   // the buffer is free (all warps leave the same sequences in the same order)
-  put(s, l0, l1, part + (warp / G) * rec_floats(H), H, (warp % G) * GROUP, lane);
+  put(s, part + (warp / G) * rec_floats(H), H, (warp % G) * GROUP, lane);
   consumers_sync();
   for (int i = threadIdx.x; i < H * D / 2; i += NW * 32) {
     const int h = i / (D / 2);
