@@ -90,20 +90,21 @@ constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 struct Rows {
   uint32_t qb[4][2];    // B operand of S^T: query codes' partners, fp16
   float qs0, qs1;       // 2^-24 sum of the scaled query row
+  float scale;          // sm_scale in log2 units
   float o[4][4];        // sums of w s c 2^-24 (rows r), of w s 16 c 2^-24 (rows r + 8)
   float z0, z1;         // this lane's sums of w m
   // pairs, of head 2t and head 2t + 1, the same in a head's lanes:
-  uint64_t kq;          // u kq is the logit in log2 units, u = s (q . c) + m sum q
+  uint64_t kq;          // a power of two: u kq is the logit in log2 units, u = scale (s (q . c) + m sum q)
   uint64_t nm;          // minus a recent maximum of the logits, rounded up to an integer (NO_MAX: none yet)
-  uint64_t lift;        // w = p 2^lift, p = 2^(u kq - m); every w s so far is below 2^16
-  uint64_t l;           // this lane's sums of w
+  uint64_t f;           // 2^lift: w = p 2^lift, p = 2^(u kq - m); every w s so far is below 2^16
+  uint64_t l;           // this lane's sums of p
   __nv_bfloat162 bound; // V scales and magnitudes of minima up to here are taken with p up to 2^ROOM_P
 };
 
-constexpr float NO_MAX = -1e30f;     // below every logit that is not -inf
+constexpr float NO_MAX = -3.402823466e38f;   // no logit is below, but for -inf
 // log2 of what w s may reach, of how far p may pass 1 and a scale the one that
 // the lift was chosen by before it is chosen again, and of what 2^lift may reach
-// (sums of w stay far from fp32's end).
+// (w stays far from fp32's end).
 constexpr int TOP = 15, ROOM_P = 3, ROOM_S = 4, MAX_LIFT = 105;
 // A row of one value has scale 0: 2^OF_MIN of its minimum counts as its scale, so that
 // w m stays below 2^76.  (A scale that is not 0 is at least 2^-12 of the minimum.)
@@ -120,7 +121,7 @@ __device__ __forceinline__ void clear(Rows& s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) s.o[i][0] = s.o[i][1] = s.o[i][2] = s.o[i][3] = 0.f;
   s.nm = pair(-NO_MAX, -NO_MAX);
-  s.lift = pair(MAX_LIFT, MAX_LIFT);
+  s.f = pair(pow2_bits(127 + MAX_LIFT), pow2_bits(127 + MAX_LIFT));
   s.bound = bound_of(MAX_LIFT);
   s.l = pair(0.f, 0.f);
   s.z0 = s.z1 = 0.f;
@@ -144,6 +145,7 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
   // has it in [2^14, 2^15)
   const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 20);
   const float f = pow2_bits(268 - ex);
+  s.scale = scale_log2;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -159,7 +161,7 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
     s.qb[ks][1] = pack_f16(x[d + 1] * 0.0625f, x[d + 5] * 0.0625f);
   }
   const float qs = sum * 5.9604644775390625e-8f;               // 2^-24
-  const float kq = scale_log2 * pow2_bits(min(ex + 10, 254));  // 2^24 / f
+  const float kq = pow2_bits(min(ex + 10, 254));               // 2^24 / f
   s.qs0 = __shfl_sync(0xffffffffu, qs, 8 * t);
   s.qs1 = __shfl_sync(0xffffffffu, qs, 8 * t + 4);
   s.kq = pair(__shfl_sync(0xffffffffu, kq, 8 * t), __shfl_sync(0xffffffffu, kq, 8 * t + 4));
@@ -184,6 +186,9 @@ __device__ __forceinline__ __nv_bfloat162 magnitudes(uint32_t par) { return __ha
 
 constexpr float REST = TOP - ROOM_P - ROOM_S;
 
+// log2 of a power of two.
+__device__ __forceinline__ float log2_of(float pow2) { return static_cast<float>(static_cast<int>(__float_as_uint(pow2) >> 23) - 127); }
+
 // The running state moved so that the maxima cover x0 kq and x1 kq (this lane's
 // largest logits) and every w s of the tile (logits u kq, V parameters vp) is at
 // most 2^REST.
@@ -193,15 +198,17 @@ __device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const ui
     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
     x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
   }
-  float kq0, kq1, m0, m1, lift0, lift1;
+  float kq0, kq1, m0, m1, f0, f1, l0, l1;
   split(s.kq, kq0, kq1);
   x0 *= kq0;
   x1 *= kq1;
   split(s.nm, m0, m1);
-  split(s.lift, lift0, lift1);
+  split(s.f, f0, f1);
+  split(s.l, l0, l1);
   m0 = -m0;
   m1 = -m1;
   const float n0 = fmaxf(m0, ceilf(x0)), n1 = fmaxf(m1, ceilf(x1));
+  const float lift0 = log2_of(f0), lift1 = log2_of(f1);
   float r0 = -INFINITY, r1 = -INFINITY;   // log2 of the tile's largest p s
 #pragma unroll
   for (int i = 0; i < 2 * PPW; ++i) {
@@ -218,16 +225,16 @@ __device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const ui
   // What was added before is below 2^(TOP + m - n) now; the lift may rise again by as much.
   const float t0 = fminf(fminf(lift0 + (n0 - m0), static_cast<float>(MAX_LIFT)), floorf(REST - r0));
   const float t1 = fminf(fminf(lift1 + (n1 - m1), static_cast<float>(MAX_LIFT)), floorf(REST - r1));
-  // The sums go by 2^(m - n + change of the lift), which may be further from 1
-  // than an fp32 is though their products with it are not: in steps.
+  // Sums of p go by 2^(m - n), sums of w by 2^(m - n + change of the lift), which
+  // may be further from 1 than an fp32 is though the product is not: in steps.
+  s.l = pair(l0 * fast_exp2(m0 - n0), l1 * fast_exp2(m1 - n1));
   float d0 = fmaxf(m0 - n0 + (t0 - lift0), -300.f), d1 = fmaxf(m1 - n1 + (t1 - lift1), -300.f);
   s.nm = pair(-n0, -n1);
-  s.lift = pair(t0, t1);
+  s.f = pair(fast_exp2(t0), fast_exp2(t1));
   s.bound = bound_of(fmaxf(t0, t1));
 #pragma unroll 1
   do {
     const float a0 = fast_exp2(fmaxf(d0, -100.f)), a1 = fast_exp2(fmaxf(d1, -100.f));
-    s.l = mul2(s.l, pair(a0, a1));
     s.z0 *= a0;
     s.z1 *= a1;
 #pragma unroll
@@ -262,8 +269,12 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     mma_f16(c, x8 & LOW, z8 & LOW, x8 & HIGH, z8 & HIGH, s.qb[1][0], s.qb[1][1]);
     mma_f16(c, w.y & LOW, w.w & LOW, w.y & HIGH, w.w & HIGH, s.qb[2][0], s.qb[2][1]);
     mma_f16(c, y8 & LOW, w8 & LOW, y8 & HIGH, w8 & HIGH, s.qb[3][0], s.qb[3][1]);
-    const float sa = __uint_as_float(par.x << 16), ma = __uint_as_float(par.x & 0xffff0000u);
-    const float sb = __uint_as_float(par.y << 16), mb = __uint_as_float(par.y & 0xffff0000u);
+    // With the scale in s and m, the power of two kq makes exact logits of these:
+    // a maximum can be subtracted from them in one step whatever their magnitude.
+    const uint64_t by = pair(s.scale, s.scale);
+    float sa, ma, sb, mb;
+    split(mul2(pair(__uint_as_float(par.x << 16), __uint_as_float(par.x & 0xffff0000u)), by), sa, ma);
+    split(mul2(pair(__uint_as_float(par.y << 16), __uint_as_float(par.y & 0xffff0000u)), by), sb, mb);
     u[pg][0] = va ? fmaf(sa, c[0], ma * s.qs0) : -INFINITY;
     u[pg][1] = va ? fmaf(sa, c[1], ma * s.qs1) : -INFINITY;
     u[pg][2] = vb2 ? fmaf(sb, c[2], mb * s.qs0) : -INFINITY;
@@ -302,17 +313,18 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
   }
   uint32_t pt[PPW][2];   // w s in fp16, as B operands of O^T
   float mass[2 * PPW];   // MODE SUM: this lane's share of the pages' masses, heads 2t and 2t + 1
-  const uint64_t base = add2(s.nm, s.lift);
 #pragma unroll
   for (int pg = 0; pg < PPW; ++pg) {
     float e[4];
-    split(fma2(pair(u[pg][0], u[pg][1]), s.kq, base), e[0], e[1]);
-    split(fma2(pair(u[pg][2], u[pg][3]), s.kq, base), e[2], e[3]);
+    split(fma2(pair(u[pg][0], u[pg][1]), s.kq, s.nm), e[0], e[1]);
+    split(fma2(pair(u[pg][2], u[pg][3]), s.kq, s.nm), e[2], e[3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = fast_exp2(e[i]);
     const uint64_t both = add2(pair(e[0], e[1]), pair(e[2], e[3]));
     s.l = add2(s.l, both);
     if (MODE == CE_MODE_SUM) split(both, mass[2 * pg], mass[2 * pg + 1]);
+    split(mul2(pair(e[0], e[1]), s.f), e[0], e[1]);
+    split(mul2(pair(e[2], e[3]), s.f), e[2], e[3]);
     const float sa = __uint_as_float(vp[pg].x << 16), ma = __uint_as_float(vp[pg].x & 0xffff0000u);
     const float sb = __uint_as_float(vp[pg].y << 16), mb = __uint_as_float(vp[pg].y & 0xffff0000u);
     s.z0 = fmaf(e[0], ma, fmaf(e[2], mb, s.z0));
@@ -356,7 +368,7 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
     const int pg = r >> 2, h = (r >> 1) & 1;
     if (!(r & 1) && (!TAIL || pg * P < ntok) && side.cpos + pg < side.capacity) {
       float n0, n1;
-      split(base, n0, n1);
+      split(s.nm, n0, n1);
       side.ul[(side.cpos + pg) * side.H + side.hcol + h] = y > 0.f ? __log2f(y) - (h ? n1 : n0) : -INFINITY;
     }
   }
@@ -388,7 +400,7 @@ __device__ __forceinline__ void stage(Rows& s, const uint8_t* kb, const uint8_t*
 // h0 .. h0 + 7 of a record-shaped buffer of H heads.
 __device__ __forceinline__ void put(Rows& s, float* rec, int H, int h0, int lane) {
   const int r = lane >> 2, t = lane & 3;
-  float l0, l1, m0, m1, lift0, lift1;
+  float l0, l1, m0, m1, f0, f1;
   split(s.l, l0, l1);
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
@@ -398,22 +410,23 @@ __device__ __forceinline__ void put(Rows& s, float* rec, int H, int h0, int lane
     s.z1 += __shfl_xor_sync(0xffffffffu, s.z1, o);
   }
   split(s.nm, m0, m1);
-  split(s.lift, lift0, lift1);
+  split(s.f, f0, f1);
+  const float down0 = fast_exp2(-log2_of(f0)), down1 = fast_exp2(-log2_of(f1));
   const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
   float* o = rec + (h0 + 2 * t) * D + r;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    o[q * 16] = fmaf(s.o[q][0], 16777216.f, s.z0) * i0;
-    o[D + q * 16] = fmaf(s.o[q][1], 16777216.f, s.z1) * i1;
-    o[q * 16 + 8] = fmaf(s.o[q][2], 1048576.f, s.z0) * i0;
-    o[D + q * 16 + 8] = fmaf(s.o[q][3], 1048576.f, s.z1) * i1;
+    o[q * 16] = fmaf(s.o[q][0], 16777216.f, s.z0) * i0 * down0;
+    o[D + q * 16] = fmaf(s.o[q][1], 16777216.f, s.z1) * i1 * down1;
+    o[q * 16 + 8] = fmaf(s.o[q][2], 1048576.f, s.z0) * i0 * down0;
+    o[D + q * 16 + 8] = fmaf(s.o[q][3], 1048576.f, s.z1) * i1 * down1;
   }
   if (r == 0) {
     float* ml = rec + H * D + (h0 + 2 * t) * 2;
-    ml[0] = m0 == -NO_MAX ? -INFINITY : -m0;
-    ml[1] = l0 * fast_exp2(-lift0);
-    ml[2] = m1 == -NO_MAX ? -INFINITY : -m1;
-    ml[3] = l1 * fast_exp2(-lift1);
+    ml[0] = l0 == 0.f ? -INFINITY : -m0;
+    ml[1] = l0;
+    ml[2] = l1 == 0.f ? -INFINITY : -m1;
+    ml[3] = l1;
   }
 }
 

@@ -170,3 +170,50 @@ def test_long_rows_in_one_block(G):
         tol = (2.0 ** -8 * mean.abs() + (2.0 ** -19 + (n / 32 + 64) * 2.0 ** -24) * above + (n / 8 + 64) * 2.0 ** -24 * low)
         off = ((out[:, 8 * g:8 * g + 8] - mean).abs() / tol).view(B, 8, 4, 2, 8).amax((0, 1, 2, 4))
         assert (off <= 1).all(), (g, off)      # dims 0 .. 7 and 8 .. 15 of every 16
+
+
+@pytest.mark.parametrize("G,n", [(1, 700), (8, 2011)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_logits_of_any_magnitude(sign, G, n):
+    """Logits (1 + c) 2^e / 8 with c the first code of a key, e from 6 to 116 by
+    head, up or down: three keys share the largest one exactly, the next is
+    2^e / 8 below, so the output is the mean of three value rows, whose scales
+    are 2^-20, 1 and 2^20, within the fp16 rounding of each and the output's."""
+    gen = torch.Generator().manual_seed(9)
+    units = -(-n // 16)
+    best = [5, n // 2, n - 1]
+    code = torch.randint(0, 16, (units * 16, G, 64), generator=gen)
+    first = torch.randint(0, 15, (units * 16, G), generator=gen)
+    first[best] = 15
+    code[..., 0] = first if sign > 0 else 15 - first
+    one = torch.ones((units, G, 16), dtype=torch.bfloat16)
+    paged = lambda x: x.view(units, 16, G, -1).transpose(1, 2)
+    kp = ref.pack(paged(code).to(torch.uint8), one, one, True)
+    v = torch.randn((n, G, 64), generator=gen)
+    for at, power in zip(best, (-20, 0, 20)):
+        v[at] *= 2.0 ** power
+    vp = slices(v.to(torch.bfloat16), False)
+    power = torch.tensor([6.0, 10.0, 22.0, 25.0, 28.0, 34.0, 60.0, 116.0]).repeat(G)
+    q = torch.zeros((8 * G, 64))
+    q[:, 0] = sign * 2.0 ** power
+    out, lse = one_row(q.to(torch.bfloat16), kp, vp, n)
+    top = sign * 2.0 ** power.double() / 8 * (16 if sign > 0 else 1) + math.log(3)
+    alone = torch.arange(8 * G) % 8 > 0            # 2^6 / 8 = 8 apart, e^-8: the first head sees others
+    assert ((lse - top).abs() <= 2.0 ** -21 * (1 + top.abs()))[alone].all()
+    for g in range(G):
+        c, s, m = (x.reshape(-1, x.shape[-1])[best] for x in ref.unpack(vp[:, g], False))
+        mean = (m + c * s).mean(0)
+        tol = 2.0 ** -8 * mean.abs() + 2.0 ** -11 * (c * s).mean(0) + 2.0 ** -20 * (c * s + m.abs()).mean(0)
+        got = out[8 * g + 1:8 * g + 8]
+        assert ((got - mean).abs() <= tol).all(), ((got - mean).abs() / tol).amax(-1)
+    hold(q.to(torch.bfloat16)[::8].repeat_interleave(8, 0), kp, vp, n)
+
+
+@pytest.mark.parametrize("G,n", [(1, 700), (8, 2011)])
+def test_value_scales_near_the_end_of_the_range(G, n):
+    """V scales beyond 2^68 and up to 2^122, where the weights of keys that count
+    for the normaliser would leave fp32 if the sum shared the values' lift."""
+    q, k, v = draws(n, G, 10)
+    for power in (70, 100, 120):
+        x = (v * 2.0 ** power).to(torch.bfloat16)
+        hold(q, slices(k, True), slices(x, False), n)
