@@ -142,10 +142,16 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   // exponent field of the row's largest magnitude; the row times 2^(14 - e)
-  // has it in [2^14, 2^15)
-  const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 20);
+  // has it in [2^14, 2^15).  Beside queries from 2^73 on, 2^k of what that power
+  // takes away goes into the scale, which meets keys that are small then: into
+  // the logits at the end it would pass fp32's end.
+  int ex = static_cast<int>(__float_as_uint(top) >> 23), most = ex;
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const int k = max(0, most - 200);
+  ex = max(ex, 20 + k);
   const float f = pow2_bits(268 - ex);
-  s.scale = scale_log2;
+  s.scale = scale_log2 * pow2_bits(127 + k);
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -161,7 +167,7 @@ __device__ __forceinline__ void load_query(Rows& s, const __nv_bfloat16* q, int 
     s.qb[ks][1] = pack_f16(x[d + 1] * 0.0625f, x[d + 5] * 0.0625f);
   }
   const float qs = sum * 5.9604644775390625e-8f;               // 2^-24
-  const float kq = pow2_bits(min(ex + 10, 254));               // 2^24 / f
+  const float kq = pow2_bits(ex + 10 - k);                     // 2^24 / (f 2^k)
   s.qs0 = __shfl_sync(0xffffffffu, qs, 8 * t);
   s.qs1 = __shfl_sync(0xffffffffu, qs, 8 * t + 4);
   s.kq = pair(__shfl_sync(0xffffffffu, kq, 8 * t), __shfl_sync(0xffffffffu, kq, 8 * t + 4));

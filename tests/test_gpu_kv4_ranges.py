@@ -217,3 +217,12 @@ def test_value_scales_near_the_end_of_the_range(G, n):
     for power in (70, 100, 120):
         x = (v * 2.0 ** power).to(torch.bfloat16)
         hold(q, slices(k, True), slices(x, False), n)
+
+
+@pytest.mark.parametrize("G", [1, 8])
+@pytest.mark.parametrize("power", [110, 117, 118, 121, 125])
+def test_query_rows_near_the_largest_bf16(power, G):
+    """Query rows of 2^power times ordinary values against keys of 2^-power."""
+    q, k, v = draws(700, G, 11)
+    q = (q.float() / 4 * 2.0 ** power).to(torch.bfloat16)
+    hold(q, slices((4 * k.float() * 2.0 ** -power).to(torch.bfloat16), True), slices(v.to(torch.bfloat16), False), 700)
