@@ -68,7 +68,9 @@ __device__ __forceinline__ void encode(const uint32_t (&w)[4], float lo, float s
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) {
       const uint32_t x = i < 4 ? (i < 2 ? w[0] : w[1]) : (i < 6 ? w[2] : w[3]);
-      const uint32_t c = divide(__uint_as_float((i & 1) ? x & 0xffff0000u : x << 16) - lo, s);
+      const float v = __uint_as_float((i & 1) ? x & 0xffff0000u : x << 16);
+      // (halves of the large ones, exact, where the span lies beyond fp32's end)
+      const uint32_t c = s > 1.f ? divide(v * 0.5f - lo * 0.5f, s * 0.5f) : divide(v - lo, s);
       if (i < 4) a |= c << (8 * i);
       else b |= c << (8 * i - 32);
     }

@@ -6,7 +6,8 @@
 // scale s and a minimum m, the value being m + c * s:
 //   m = min(x)                 (exact: a bf16 input)
 //   s = bf16((max / 2 - min / 2) * (2 / 15))      (halves, so that it cannot overflow)
-//   c = clamp(rint((x - m) / s), 0, 15)           (fp32, ties to even; 0 where s is 0)
+//   c = clamp(rint((x - m) / s), 0, 15)           (fp32, ties to even; 0 where s is 0;
+//                                                  by halves where x - m is beyond fp32)
 // The scale's rounding to bf16 moves the top code by at most 15 * 2^-9 of a
 // step.  A row that holds a NaN or an infinity is kept as s = m = NaN, c = 0.
 //

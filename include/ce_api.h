@@ -458,7 +458,8 @@ int ce_reservoir_scores(const int32_t* pos, int32_t layers, int32_t heads,
  * CE_KV4_SLICE_BYTES (576 instead of 2,048) bytes, 16-byte aligned.  Of each
  * (token, KV head) row x of 64 values it keeps
  *   m = min(x), s = bf16((max / 2 - min / 2) * (2 / 15)),
- *   c = clamp(rint((x - m) / s), 0, 15)   (fp32, ties to even; 0 where s = 0)
+ *   c = clamp(rint((x - m) / s), 0, 15)   (fp32, ties to even; 0 where s = 0;
+ *                                          by halves where x - m is beyond fp32)
  * and a value is m + c * s.  A row with a NaN or an infinity reads as NaN
  * throughout.  Bytes 0..511 of a slice hold the codes, bytes 512 + 4 j the
  * scale and then the minimum (bf16) of token j:
