@@ -143,5 +143,6 @@ extern "C" int ce_prepare_device(void) {
   if (st == CE_OK) st = ce::host::fill_prepare_device();
   if (st == CE_OK) st = ce::host::pool_prepare_device();
   if (st == CE_OK) st = ce::host::kv4_prepare_device();
+  if (st == CE_OK) st = ce::host::window_prepare_device();
   return st;
 }

@@ -79,5 +79,8 @@ int pool_prepare_device();
 int kv4_prepare_device();
 int kv4_copy_prepare_device();
 
+// The same for the windowed prefill kernels (ce_window.cu).
+int window_prepare_device();
+
 }  // namespace host
 }  // namespace ce

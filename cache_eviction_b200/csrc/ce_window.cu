@@ -871,12 +871,17 @@ extern "C" int ce_window_prefill(const void* q, int64_t q_st, int64_t q_sh, cons
   p.o_st = o_st;
   p.o_sh = o_sh;
   p.err = err;
-  if (!host::set_smem(attend_kernel<16>, SMEM) || !host::set_smem(attend_kernel<0>, SMEM))
-    return host::fail(CE_ERR_CUDA, "ce_window_prefill: smem attr");
+  if (host::window_prepare_device() != CE_OK) return CE_ERR_CUDA;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.items, sms));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (page_size == 16) attend_kernel<16><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
   else attend_kernel<0><<<grid, THREADS, SMEM, st>>>(p, qmap, kmap, vmap);
   if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("ce_window_prefill launch");
+  return CE_OK;
+}
+
+int ce::host::window_prepare_device() {
+  if (!set_smem(window::attend_kernel<16>, window::SMEM) || !set_smem(window::attend_kernel<0>, window::SMEM))
+    return fail_cuda("windowed prefill kernels: set-up");
   return CE_OK;
 }

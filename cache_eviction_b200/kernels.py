@@ -649,8 +649,9 @@ def boundary(table, req_to_unit, frontier, count, pos, scores, k_ptrs, v_ptrs, k
 
 
 def prepare_device(device):
-    """Load the library's decode, boundary, CSR and pool kernels on `device`
-    (ce_prepare_device), so that no later call pays the module load."""
+    """Load the library's decode, boundary, CSR, pool, 4-bit and windowed kernels
+    on `device` (ce_prepare_device), so that no later call of theirs pays the
+    module load."""
     with torch.cuda.device(torch.device(device)):
         capi.check(capi.load().ce_prepare_device(), "ce_prepare_device")
 

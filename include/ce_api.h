@@ -99,7 +99,8 @@ const char* ce_status_string(int status);
 /* Detail of the last failing call made by this host thread. */
 const char* ce_last_error(void);
 
-/* Load the decode, selection / boundary, CSR and unit-pool kernels on the
+/* Load the decode (bf16, windowed and 4-bit), selection / boundary, CSR,
+ * unit-pool, 4-bit write and read-back and windowed prefill kernels on the
  * current device and set their launch attributes, which their entry points
  * otherwise do on first use.  Under lazy module loading (the CUDA 12 default)
  * a first ce_boundary call spends ~5 ms loading its kernels; a server calls
