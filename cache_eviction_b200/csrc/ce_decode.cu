@@ -56,6 +56,30 @@ constexpr int SMEM_BYTES = NSTAGES * STAGE_BYTES + 1024 /*align*/ + 1024 /*barri
 
 constexpr int MIN_STAGES_LOG2 = 2;        // at least 4 stages per CTA: the pipeline's depth
 
+// When there are fewer stages than CTAs some partitions are empty and leave
+// no record; a sequence's record range [k0, k1] may straddle them.
+__device__ __forceinline__ bool cta_has_work(int64_t k, int64_t S, int64_t grid) {
+  return (k * S) / grid < ((k + 1) * S) / grid;
+}
+
+__device__ __forceinline__ void store_out(const Params& p, int b, int h, int d, float v) {
+  const int64_t off = static_cast<int64_t>(b) * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d;
+  if (p.out_f32)
+    reinterpret_cast<float*>(p.out)[off] = v;
+  else
+    reinterpret_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
+}
+
+// A sequence with no tokens attends only to the sink: zero output.
+__device__ __forceinline__ void empty_sequence(const Params& p, int b) {
+  for (int h = 0; h < p.H; ++h) {
+    for (int d = 0; d < D; ++d) store_out(p, b, h, d, 0.f);
+    const float s2 = p.sinks ? p.sinks[h] * LOG2E : -INFINITY;
+    p.lse2[static_cast<int64_t>(b) * p.H + h] = s2;
+    if (p.lse_out) p.lse_out[static_cast<int64_t>(b) * p.H + h] = s2 * LN2;
+  }
+}
+
 __device__ __forceinline__ int stage_tokens(int G) { return 16 * (NCW / G); }
 
 // Stages of a sequence of n tokens.  WIN: only those that hold a visible
@@ -773,7 +797,7 @@ __global__ void __launch_bounds__(CB_THREADS, SB == 1 ? 4 : 2) combine_kernel(co
   const Params& p = cp.a;
   const int bs = p.bs, H = p.H, G = p.G, C = cp.chunks;
   const int64_t S = p.prefix[bs];
-  const int64_t grid = eff_grid(S, cp.grid, p.min_log2);
+  const int64_t grid = eff_grid(S, cp.grid, MIN_STAGES_LOG2);
   const int hgroups = H / GROUP;
   const int64_t ntasks = static_cast<int64_t>(bs) * hgroups * C;
   __shared__ float sh_m[GROUP * CB_THREADS], sh_l[GROUP * CB_THREADS];
@@ -913,28 +937,6 @@ host::DecodeLayout ce::host::decode_layout(int bs, int64_t cap, int H, int P, in
   return L;
 }
 
-int ce::host::launch_combine(const Params& p, int grid, int P, bool defer, cudaStream_t st) {
-  const int sms = sm_count();
-  CombineParams cp{p, grid, P, defer ? 1 : 0, combine_chunks(p.bs, p.H, sms)};
-  const int64_t tasks = static_cast<int64_t>(p.bs) * (p.H / GROUP) * cp.chunks;
-  const int cb_grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tasks, 4LL * sms)));
-  // Fewer (sequence, KV head) pairs than SMs: each head has many record slots
-  // (up to one per CTA and warp group) and the tasks are chunks of few
-  // sequences -- the wide variant's batched loads win.
-  // A deferred decode's page scores run beside the next layer's attention
-  // kernel (195 KB of shared memory per CTA): keep SMs at the largest carveout.
-  const bool wide = static_cast<int64_t>(p.bs) * (p.H / GROUP) < sms;
-  if (wide) {
-    if (defer && !set_max_shared_carveout(combine_kernel<CB_SLOT_BATCH_WIDE>)) return fail(CE_ERR_CUDA, "carveout attr");
-    combine_kernel<CB_SLOT_BATCH_WIDE><<<cb_grid, CB_THREADS, 0, st>>>(cp);
-  } else {
-    if (defer && !set_max_shared_carveout(combine_kernel<1>)) return fail(CE_ERR_CUDA, "carveout attr");
-    combine_kernel<1><<<cb_grid, CB_THREADS, 0, st>>>(cp);
-  }
-  if (cudaPeekAtLastError() != cudaSuccess) return fail_cuda("combine_kernel launch");
-  return CE_OK;
-}
-
 extern "C" int64_t ce_decode_workspace_bytes(int32_t bs, int64_t kv_capacity, int32_t num_q_heads,
                                              int32_t num_kv_heads, int32_t page_size,
                                              int32_t score_flags) {
@@ -946,6 +948,31 @@ extern "C" int64_t ce_decode_workspace_bytes(int32_t bs, int64_t kv_capacity, in
 }
 
 namespace {
+
+// Merges the records that an attention launch of `grid` CTAs left for the
+// batch of p into outputs, log normalisers and (unless deferred) page scores.
+// Returns a CE_* status.
+int launch_combine(const Params& p, int grid, int P, bool defer, cudaStream_t st) {
+  const int sms = host::sm_count();
+  CombineParams cp{p, grid, P, defer ? 1 : 0, combine_chunks(p.bs, p.H, sms)};
+  const int64_t tasks = static_cast<int64_t>(p.bs) * (p.H / GROUP) * cp.chunks;
+  const int cb_grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tasks, 4LL * sms)));
+  // Fewer (sequence, KV head) pairs than SMs: each head has many record slots
+  // (up to one per CTA and warp group) and the tasks are chunks of few
+  // sequences -- the wide variant's batched loads win.
+  // A deferred decode's page scores run beside the next layer's attention
+  // kernel (195 KB of shared memory per CTA): keep SMs at the largest carveout.
+  const bool wide = static_cast<int64_t>(p.bs) * (p.H / GROUP) < sms;
+  if (wide) {
+    if (defer && !host::set_max_shared_carveout(combine_kernel<CB_SLOT_BATCH_WIDE>)) return host::fail(CE_ERR_CUDA, "carveout attr");
+    combine_kernel<CB_SLOT_BATCH_WIDE><<<cb_grid, CB_THREADS, 0, st>>>(cp);
+  } else {
+    if (defer && !host::set_max_shared_carveout(combine_kernel<1>)) return host::fail(CE_ERR_CUDA, "carveout attr");
+    combine_kernel<1><<<cb_grid, CB_THREADS, 0, st>>>(cp);
+  }
+  if (cudaPeekAtLastError() != cudaSuccess) return host::fail_cuda("combine_kernel launch");
+  return CE_OK;
+}
 
 // WIN: only the window's tokens and the first ones are visible, and nothing is scored.
 template <int P, bool WIN>
@@ -1023,7 +1050,6 @@ int decode_call(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool, c
   p.rec = reinterpret_cast<float*>(ws + L.rec);
   p.ul = (score_flags & 3) ? reinterpret_cast<float*>(ws + L.ul) : nullptr;
   p.tl = ((score_flags & 2) && page_size > 1) ? reinterpret_cast<float*>(ws + L.tl) : nullptr;
-  p.min_log2 = MIN_STAGES_LOG2;
   p.window = window;
   p.first = first;
   p.err = err;
@@ -1032,7 +1058,7 @@ int decode_call(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pool, c
   const int launched = page_size == 16 ? launch_attn<16, WIN>(grid, kmap, vmap, p, st)
                                        : launch_attn<1, WIN>(grid, kmap, vmap, p, st);
   if (launched != CE_OK) return launched;
-  return host::launch_combine(p, grid, page_size, (score_flags & CE_SCORE_DEFER) != 0, st);
+  return launch_combine(p, grid, page_size, (score_flags & CE_SCORE_DEFER) != 0, st);
 }
 
 }  // namespace

@@ -1,7 +1,6 @@
 // Shared by the decode kernels (bf16 pages: ce_decode.cu, 4-bit pages:
 // ce_kv4_decode.cu): the parameters of a decode call, the split of a batch
-// into stages, the partial records that attention CTAs leave, the workspace
-// and the combine launch that merges the records.
+// into stages over CTAs and the workspace.
 #pragma once
 
 #include <cuda.h>
@@ -47,7 +46,6 @@ struct Params {
   float* rec;        // [(bs + grid), REC_FLOATS]
   float* ul;         // [kv_capacity, H] unit log-mass (log2 units) or null
   float* tl;         // [kv_capacity * P, H] token logits (page_size > 1, MAX rows) or null
-  int min_log2;      // log2 of the fewest stages an attention CTA takes
   int window, first; // windowed decode: tokens t >= n - window or t < first (window < 0: all)
   int32_t* err;
 };
@@ -101,30 +99,6 @@ __device__ __forceinline__ int cta_of_stage(int64_t x, int64_t S, int64_t grid) 
   return static_cast<int>(((x + 1) * grid - 1) / S);
 }
 
-// When there are fewer stages than CTAs some partitions are empty and leave
-// no record; a sequence's record range [k0, k1] may straddle them.
-__device__ __forceinline__ bool cta_has_work(int64_t k, int64_t S, int64_t grid) {
-  return (k * S) / grid < ((k + 1) * S) / grid;
-}
-
-__device__ __forceinline__ void store_out(const Params& p, int b, int h, int d, float v) {
-  const int64_t off = static_cast<int64_t>(b) * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d;
-  if (p.out_f32)
-    reinterpret_cast<float*>(p.out)[off] = v;
-  else
-    reinterpret_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
-}
-
-// A sequence with no tokens attends only to the sink: zero output.
-__device__ __forceinline__ void empty_sequence(const Params& p, int b) {
-  for (int h = 0; h < p.H; ++h) {
-    for (int d = 0; d < D; ++d) store_out(p, b, h, d, 0.f);
-    const float s2 = p.sinks ? p.sinks[h] * LOG2E : -INFINITY;
-    p.lse2[static_cast<int64_t>(b) * p.H + h] = s2;
-    if (p.lse_out) p.lse_out[static_cast<int64_t>(b) * p.H + h] = s2 * LN2;
-  }
-}
-
 }  // namespace decode
 
 namespace host {
@@ -135,11 +109,6 @@ struct DecodeLayout {
   size_t prefix, lse2, ul, tl, rec, total;
 };
 DecodeLayout decode_layout(int bs, int64_t cap, int H, int P, int flags, int grid);
-
-// Merges the records that an attention launch of `grid` CTAs left for the
-// batch of p into outputs, log normalisers and (unless deferred) page scores.
-// Returns a CE_* status.
-int launch_combine(const decode::Params& p, int grid, int P, bool defer, cudaStream_t st);
 
 }  // namespace host
 }  // namespace ce

@@ -56,6 +56,7 @@ constexpr int MIN_STAGES_LOG2 = 0;                   // every CTA below min(stag
 
 // Floats of a record: the means of V [H][64], then (maximum, sum of p) [H].
 __host__ __device__ constexpr int rec_floats(int H) { return H * (D + 2); }
+static_assert(rec_floats(NW * GROUP) <= decode::REC_FLOATS, "the workspace's records hold it");
 
 // D += A(16x16) * B(16x8) in fp16 with fp32 accumulation.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -481,37 +482,6 @@ __device__ __forceinline__ void leave(const Params& p, Rows& s, int b, int warp,
     }
   }
 }
-
-// The batch's stages in order: sequence b from stage `base` on, its tokens and
-// first CSR position; the next sequence's are loaded one sequence ahead.
-template <int ST>
-struct Cursor {
-  int b, base, tok, nst, next_tok;
-  int64_t ip, next_ip;
-  __device__ __forceinline__ void fetch_next(const Params& p) {
-    const bool more = b + 1 < p.bs;
-    next_tok = more ? decode::seq_tokens(p, b + 1, P) : 0;
-    next_ip = more ? p.kv_indptr[b + 1] : 0;
-  }
-  __device__ __forceinline__ void start(const Params& p, int bb, int first) {
-    b = bb;
-    base = first;
-    tok = b < p.bs ? decode::seq_tokens(p, b, P) : 0;
-    ip = b < p.bs ? p.kv_indptr[b] : 0;
-    nst = (tok + ST - 1) / ST;
-    fetch_next(p);
-  }
-  __device__ __forceinline__ void to(const Params& p, int x) {   // x below the batch's stages
-    while (x >= base + nst) {
-      base += nst;
-      ++b;
-      tok = next_tok;
-      ip = next_ip;
-      nst = (tok + ST - 1) / ST;
-      fetch_next(p);
-    }
-  }
-};
 
 // Sizes that go with G KV heads: a stage is WT tokens of every consumer warp.
 // Below 8 heads several warps share a head and leave() needs a buffer, so
@@ -1090,8 +1060,6 @@ extern "C" int ce_kv4_decode_attn_score(const void* q, int64_t q_sb, int64_t q_s
   p.rec = reinterpret_cast<float*>(ws + L.rec);
   p.ul = (score_flags & 3) ? reinterpret_cast<float*>(ws + L.ul) : nullptr;
   p.tl = (score_flags & 2) ? reinterpret_cast<float*>(ws + L.tl) : nullptr;
-  p.min_log2 = kv4::MIN_STAGES_LOG2;
-  p.window = -1;
   p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint8_t *kp = static_cast<const uint8_t*>(k_pool), *vp = static_cast<const uint8_t*>(v_pool);
