@@ -416,6 +416,21 @@ __device__ __forceinline__ float weights(const float (&v)[32], float scale2, flo
   return a + b;
 }
 
+// A weight's exponent, scale2 v - m, is one rounding of the exact product, so at
+// the maximum it is what m was rounded by: from 2^30 on that could leave fp32.
+// There a row's scale is cut by a power of two that keeps m below 2^30: logits
+// that differ at all differ by 32 octaves still.  Old and new maximum m and mt
+// (in units of the scale so far) and the scale for a maximum that rises to mt.
+constexpr float FAR = 1073741824.f;
+__device__ __forceinline__ void rescale(float& m, float& mt, float& scale2, float full) {
+  const float cut = full / scale2, now = mt * cut;   // in log2 units
+  const int over = max(0, static_cast<int>(__float_as_uint(fabsf(now)) >> 23) - (127 + 29));
+  const float by = __uint_as_float(static_cast<uint32_t>(127 - over) << 23);
+  m = fmaxf(m * cut * by, now * by - FAR);           // (no further below than what makes a factor 0)
+  mt = now * by;
+  scale2 = full * by;
+}
+
 // The two warps of a query tile's row quarter (named barriers 1 to 8).
 __device__ __forceinline__ void quarter_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id + 1) : "memory"); }
 // Turns at the exponentials (named barriers 9 and 10): query tile x waits for
@@ -651,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         Span own = sp;
         own.p_lo = it.prefix + min(it.q0 + tile * QT + quarter * 4, it.nq - 1);
         own.p_hi = it.prefix + min(it.q0 + tile * QT + quarter * 4 + 3, it.nq - 1);
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, scale2 = p.scale2;
         for (int t = 0; t < ntiles; ++t, ++n) {
           ok = ok && warp_wait_quiet(&sy->sfull[tile], n & 1, p.err, abort, lane);
           float mt = -INFINITY;
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[i + 2 * k], v[i + 2 * k + 1]);
             }
-            mt = p.scale2 * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            mt = scale2 * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             top[n & 1][half][r] = mt;
           }
           quarter_sync(tile * 4 + quarter);
@@ -698,6 +713,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_after();
           const bool grow = mt > m + LAZY || (m == -INFINITY && mt > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
+            if (grow && (fabsf(mt) >= FAR || scale2 != p.scale2)) rescale(m, mt, scale2, p.scale2);
             const float mn = grow ? mt : m;
             const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
             l *= a;
@@ -726,7 +742,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               __syncwarp();
               if (lane == 0) mbar_arrive(&sy->sempty[tile]);
             }
-            l += weights(v, p.scale2, mu, pcol + c / 2);
+            l += weights(v, scale2, mu, pcol + c / 2);
           }
           if (groups == 2) turn_give(tile ^ 1);
           tmem_st_wait();
@@ -740,7 +756,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         sy->sum[tile][half][r] = l;
         quarter_sync(tile * 4 + quarter);
         l += sy->sum[tile][half ^ 1][r];
-        if (p.sinks) l += exp2f(sink - m);
+        if (p.sinks) l += exp2f(sink - m * (p.scale2 / scale2));
         float f = 1.f / l;
         ok = ok && warp_wait_quiet(&sy->odone[tile], done & 1, p.err, abort, lane);
         ++done;
