@@ -114,7 +114,7 @@ constexpr int OF_MIN = -60;
 // The bound that goes with the larger of a lane's two lifts.
 __device__ __forceinline__ __nv_bfloat162 bound_of(float lift) {
   const int e = 127 + TOP - ROOM_P - static_cast<int>(lift);
-  const uint32_t b = static_cast<uint32_t>(min(e, 255) << 7 | min(e - OF_MIN, 255) << 23);   // (infinite from 2^128 on)
+  const uint32_t b = static_cast<uint32_t>(min(e, 254) << 7 | min(e - OF_MIN, 254) << 23);
   return *reinterpret_cast<const __nv_bfloat162*>(&b);
 }
 
@@ -194,7 +194,11 @@ __device__ __forceinline__ __nv_bfloat162 magnitudes(uint32_t par) { return __ha
 constexpr float REST = TOP - ROOM_P - ROOM_S;
 
 // log2 of a power of two.
-__device__ __forceinline__ float log2_of(float pow2) { return static_cast<float>(static_cast<int>(__float_as_uint(pow2) >> 23) - 127); }
+__device__ __forceinline__ int log2_of(float pow2) { return static_cast<int>(__float_as_uint(pow2) >> 23) - 127; }
+// What counts as a token's scale.
+__device__ __forceinline__ float reach(float scale, float minimum) {
+  return fmaxf(scale, fabsf(minimum) * pow2_bits(127 + OF_MIN));
+}
 
 // The running state moved so that the maxima cover x0 kq and x1 kq (this lane's
 // largest logits) and every w s of the tile (logits u kq, V parameters vp) is at
@@ -220,7 +224,7 @@ __device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const ui
 #pragma unroll
   for (int i = 0; i < 2 * PPW; ++i) {
     const uint32_t par = i & 1 ? vp[i / 2].y : vp[i / 2].x;
-    const float e = __log2f(fmaxf(__uint_as_float(par << 16), fabsf(__uint_as_float(par & 0xffff0000u)) * pow2_bits(127 + OF_MIN)));
+    const float e = __log2f(reach(__uint_as_float(par << 16), __uint_as_float(par & 0xffff0000u)));
     r0 = fmaxf(r0, u[i / 2][2 * (i & 1)] * kq0 - n0 + e);
     r1 = fmaxf(r1, u[i / 2][2 * (i & 1) + 1] * kq1 - n1 + e);
   }
@@ -237,7 +241,7 @@ __device__ __forceinline__ void move(Rows& s, const float (&u)[PPW][4], const ui
   s.l = pair(l0 * fast_exp2(m0 - n0), l1 * fast_exp2(m1 - n1));
   float d0 = fmaxf(m0 - n0 + (t0 - lift0), -300.f), d1 = fmaxf(m1 - n1 + (t1 - lift1), -300.f);
   s.nm = pair(-n0, -n1);
-  s.f = pair(fast_exp2(t0), fast_exp2(t1));
+  s.f = pair(pow2_bits(127 + static_cast<int>(t0)), pow2_bits(127 + static_cast<int>(t1)));   // t in MAX_LIFT .. REST - 126
   s.bound = bound_of(fmaxf(t0, t1));
 #pragma unroll 1
   do {
@@ -304,8 +308,16 @@ __device__ __forceinline__ void tile(Rows& s, const uint8_t* kb, const uint8_t* 
   {
     float a0, a1;
     split(fma2(pair(x0, x1), s.kq, s.nm), a0, a1);
-    if (__any_sync(0xffffffffu, fmaxf(a0, a1) > ROOM_P || *reinterpret_cast<const uint32_t*>(&top) != *reinterpret_cast<const uint32_t*>(&s.bound)))
-      move(s, u, vp, x0, x1);
+    const bool high = fmaxf(a0, a1) > ROOM_P;
+    if (__any_sync(0xffffffffu, high || *reinterpret_cast<const uint32_t*>(&top) != *reinterpret_cast<const uint32_t*>(&s.bound))) {
+      // A large scale alone is common where the lift goes by keys of large weight
+      // and small values: what counts is its product with the lane's largest weight.
+      float f0, f1;
+      split(s.f, f0, f1);
+      const float ws = fmaxf(a0 + log2_of(f0), a1 + log2_of(f1)) + __log2f(reach(__low2float(top), __high2float(top)));
+      if (__any_sync(0xffffffffu, high || ws > TOP))
+        move(s, u, vp, x0, x1);
+    }
   }
   if (MODE == CE_MODE_MAX) {
     float kq0, kq1;
@@ -418,7 +430,7 @@ __device__ __forceinline__ void put(Rows& s, float* rec, int H, int h0, int lane
   }
   split(s.nm, m0, m1);
   split(s.f, f0, f1);
-  const float down0 = fast_exp2(-log2_of(f0)), down1 = fast_exp2(-log2_of(f1));
+  const float down0 = pow2_bits(127 - log2_of(f0)), down1 = pow2_bits(127 - log2_of(f1));
   const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
   float* o = rec + (h0 + 2 * t) * D + r;
 #pragma unroll

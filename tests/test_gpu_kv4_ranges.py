@@ -226,3 +226,18 @@ def test_query_rows_near_the_largest_bf16(power, G):
     q, k, v = draws(700, G, 11)
     q = (q.float() / 4 * 2.0 ** power).to(torch.bfloat16)
     hold(q, slices((4 * k.float() * 2.0 ** -power).to(torch.bfloat16), True), slices(v.to(torch.bfloat16), False), 700)
+
+
+@pytest.mark.parametrize("G,n", [(1, 700), (8, 2011)])
+@pytest.mark.parametrize("power", [-6, -12, -40])
+@pytest.mark.parametrize("logit", [3.0, 10.0, 40.0])
+def test_a_first_key_of_most_weight_and_small_values(logit, power, G, n):
+    """The first key takes most of the weight, or nearly all of it, and its
+    values are 2^power of the others'."""
+    q, k, v = draws(n, G, 12)
+    q[:, :8] = 4.0
+    k[:, :, :8] = 0.0
+    k[0] = 0.0
+    k[0, :, :8] = logit / 4.0
+    v[0] *= 2.0 ** power
+    hold(q, slices(k, True), slices(v.to(torch.bfloat16), False), n)
