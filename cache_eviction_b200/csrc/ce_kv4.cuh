@@ -8,7 +8,7 @@
 //   s = bf16((max / 2 - min / 2) * (2 / 15))      (halves, so that it cannot overflow)
 //   c = clamp(rint((x - m) / s), 0, 15)           (fp32, ties to even; 0 where s is 0;
 //                                                  by halves where x - m is beyond fp32)
-// The scale's rounding to bf16 moves the top code by at most 15 * 2^-9 of a
+// The scale's rounding to bf16 moves the top code by at most 15 * 2^-8 of a
 // step.  A row that holds a NaN or an infinity is kept as s = m = NaN, c = 0.
 //
 // Bytes 0..511 are the codes, bytes 512 + 4 j .. the scale and then the

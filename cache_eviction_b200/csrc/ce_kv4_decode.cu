@@ -27,14 +27,16 @@
 // A producer warp copies whole pages (all KV heads) into a ring of shared-memory
 // stages with untiled bulk copies; the format puts a page's fragments in lane
 // order, 16 bytes per lane and operand.  (Loading them from global memory
-// straight into registers a stage ahead needed 221 instructions per page and
-// head instead of 143 and left too few bytes in flight: 178 us instead of 102
-// for 409 MB.)
+// straight into registers a stage ahead needed 1.5 times the instructions per
+// page and left too few bytes in flight: 178 us instead of 102 for 409 MB.)
 //
-// 64 rows of 2K-32K tokens, 8 KV heads (409 MB): 88 us without scores, of which
-// the loads alone take 80 (5.1 TB/s), 121 us with sum, max and no scores mixed
-// (max scores write and read 4 KB of log-masses per page).  Copies of 576 bytes
-// bound a single KV head: 51 MB in 32 us without scores.
+// Device times.  64 rows of 2K-32K tokens, 8 KV heads (409 MB): 98 us without
+// scores (155 instructions per page and head, 58 % of the issue slots; the loads
+// alone take 80, 5.1 TB/s), 128 us with sum, max and no scores mixed (max scores
+// write and read 4 KB of log-masses per page), 1 KV head (51 MB, copies of 576
+// bytes by one warp): 34 us without scores, 45 with max scores.  Outputs of that
+// batch are 1.7e-4 (relative norm) from the same pages' in 64 bits, before their
+// rounding to bf16.
 #include <algorithm>
 
 #include "ce_decode.cuh"
